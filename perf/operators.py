@@ -39,8 +39,8 @@ def listed():
         {'name': 'muon_column', 'op': 'muon', 'shapes': COLUMN, 'vectors': '26*192,18*128,6*17'},
         # a training step of the default model, every parameter of it
         {'name': 'muon_model', 'op': 'muon', 'shapes': MODEL, 'vectors': MODEL_VECTORS},
-        # the default model's norm vectors alone
-        {'name': 'adamw_norms', 'op': 'adamw', 'shapes': MODEL_VECTORS},
+        # the norm vectors of one stage's three columns
+        {'name': 'adamw_norms', 'op': 'adamw', 'shapes': '78*192,54*128,18*17'},
         # every parameter of the default model by AdamW
         {'name': 'adamw_model', 'op': 'adamw', 'shapes': MODEL + ',' + MODEL_VECTORS},
         # one skeleton's 17 joint tokens, inference
@@ -66,7 +66,7 @@ def draw(rng):
         return {'op': 'norm', 'rows': rows, 'cols': cols, 'gap': rng.choice([0, 0, 0, 8, 5]), 'dtype': rng.choice(['float32', 'bfloat16', 'float16']),
                 'train': rng.random() < 0.7}
     if op == 'adamw':
-        shapes = ['%d*%d' % (_spread(rng, 1, 400), _spread(rng, 1, 100000)) for _ in range(rng.randint(1, 4))]
+        shapes = ['%d*%d' % (_spread(rng, 1, 100), _spread(rng, 1, 400000)) for _ in range(rng.randint(1, 4))]
         return {'op': 'adamw', 'shapes': ','.join(shapes)}
     if op == 'orth' and rng.random() < 0.4:
         m, n = _spread(rng, 64, 4096), _spread(rng, 64, 4096)
@@ -118,8 +118,17 @@ def _fill(flat, text, gen, gradients):
             v.copy_(torch.randn(v.shape, generator=gen, device=gen.device) * (1e-3 if gradients else math.sqrt(2.0 / v.shape[-1])))
 
 
-def _views(flat, text):
-    return [torch.nn.Parameter(t) for v in _groups(flat, text) for t in v.unbind(0)]
+def _tensors(flat, text):
+    return [t for v in _groups(flat, text) for t in v.unbind(0)]
+
+
+def _gather(tensors, text):
+    """Separate tensors, laid out like the arena of their parameters."""
+    flat, at = _arena(text, 'cuda'), 0
+    for v in _groups(flat, text):
+        v.copy_(torch.stack(tensors[at:at + len(v)]))
+        at += len(v)
+    return flat
 
 
 def prepare(case, seed):
@@ -145,9 +154,10 @@ def prepare(case, seed):
     matrices, vectors = (case['shapes'], case['vectors']) if case['op'] == 'muon' else ('', case['shapes'])
     s['texts'] = (matrices, vectors)
     for name, text in (('m', matrices), ('v', vectors)):
-        s['p' + name], s['g' + name] = _arena(text, 'cuda'), _arena(text, 'cuda')
+        s['p' + name], g = _arena(text, 'cuda'), _arena(text, 'cuda')
         _fill(s['p' + name], text, gen, False)
-        _fill(s['g' + name], text, gen, True)
+        _fill(g, text, gen, True)
+        s['g' + name] = [t.clone() for t in _tensors(g, text)]          # the backward pass leaves a tensor for each parameter
     s['momentum'] = _arena(matrices, 'cuda')
     _fill(s['momentum'], matrices, gen, True)
     s['momentum'] *= 8.0
@@ -158,9 +168,9 @@ def prepare(case, seed):
     s['steps'] = ADAMW_STEPS_BEFORE
     if own:          # the optimiser that a training loop keeps, in the state that it has after some steps
         from margipose_amd.train_helpers import DeviceAdamW, DeviceMuon
-        pm, pv = _views(s['pm'], matrices), _views(s['pv'], vectors)
-        for p, g in zip(pm + pv, _views(s['gm'], matrices) + _views(s['gv'], vectors)):
-            p.grad = g.detach()
+        pm, pv = ([torch.nn.Parameter(t) for t in _tensors(s['p' + k], text)] for k, text in (('m', matrices), ('v', vectors)))
+        for p, g in zip(pm + pv, s['gm'] + s['gv']):
+            p.grad = g
         adamw = {'lr': ADAMW['lr'], 'betas': (ADAMW['momentum'], ADAMW['beta2']), 'eps': ADAMW['eps'], 'weight_decay': ADAMW['weight_decay']}
         if case['op'] == 'muon':
             opt = DeviceMuon(pm, vectors=pv, ns_steps=STEPS, ns_coefficients=COEFFICIENTS, ns_eps=NS_EPS, vector_options=adamw, **MUON)
@@ -191,8 +201,9 @@ def _newton_schulz(g):
 
 def _plain_muon(s):
     h = MUON
-    s['momentum'].mul_(h['momentum']).add_(s['gm'])
-    u = s['gm'] + h['momentum'] * s['momentum']
+    g = _gather(s['gm'], s['texts'][0])
+    s['momentum'].mul_(h['momentum']).add_(g)
+    u = g + h['momentum'] * s['momentum']
     for p, v in zip(_groups(s['pm'], s['texts'][0]), _groups(u, s['texts'][0])):
         scale = 0.2 * math.sqrt(max(p.shape[1:]))
         p.mul_(1.0 - h['lr'] * h['weight_decay']).sub_(h['lr'] * scale * _newton_schulz(v))
@@ -200,10 +211,11 @@ def _plain_muon(s):
 
 def _plain_adamw(s):
     h = ADAMW
+    g = _gather(s['gv'], s['texts'][1])
     s['steps'] += 1
     b1, b2, t = h['momentum'], h['beta2'], s['steps']
-    s['exp_avg'].mul_(b1).add_((1.0 - b1) * s['gv'])
-    s['exp_avg_sq'].mul_(b2).add_((1.0 - b2) * s['gv'].square())
+    s['exp_avg'].mul_(b1).add_((1.0 - b1) * g)
+    s['exp_avg_sq'].mul_(b2).add_((1.0 - b2) * g.square())
     denominator = (s['exp_avg_sq'] / (1.0 - b2 ** t)).sqrt() + h['eps']
     s['pv'].mul_(1.0 - h['lr'] * h['weight_decay']).sub_(h['lr'] / (1.0 - b1 ** t) * s['exp_avg'] / denominator)
 
@@ -281,15 +293,16 @@ def exact(case, seed):
         return out
     if case['op'] == 'orth':
         return [_exact_orthogonal(g) for g in s['matrices']]
-    gv, pv = s['gv'].double(), s['pv'].double()
+    gv, pv = _gather(s['gv'], s['texts'][1]).double(), s['pv'].double()
     t = ADAMW_STEPS_BEFORE + 1
     m = ADAMW['momentum'] * s['exp_avg'].double() + (1.0 - ADAMW['momentum']) * gv
     v = ADAMW['beta2'] * s['exp_avg_sq'].double() + (1.0 - ADAMW['beta2']) * gv * gv
     mhat, vhat = m / (1.0 - ADAMW['momentum'] ** t), v / (1.0 - ADAMW['beta2'] ** t)
     out = {'vectors': pv - ADAMW['lr'] * (ADAMW['weight_decay'] * pv + mhat / (torch.sqrt(vhat) + ADAMW['eps'])), 'exp_avg': m, 'exp_avg_sq': v}
     if case['op'] == 'muon':
-        buf = MUON['momentum'] * s['momentum'].double() + s['gm'].double()
-        u = s['gm'].double() + MUON['momentum'] * buf
+        gm = _gather(s['gm'], s['texts'][0]).double()
+        buf = MUON['momentum'] * s['momentum'].double() + gm
+        u = gm + MUON['momentum'] * buf
         p = s['pm'].double()
         p -= MUON['lr'] * MUON['weight_decay'] * p
         for pg, ug in zip(_groups(p, case['shapes']), _groups(u, case['shapes'])):
