@@ -9,7 +9,9 @@ CSRC = os.path.join(PKG_DIR, 'csrc')
 LIB_PATH = os.path.join(PKG_DIR, 'libmargipose_hip.so')
 LOG_PATH = os.path.join(CSRC, 'build.log')      # hipcc's output of the last build, kernel-resource-usage remarks included
 HIPCC_FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++20', '-fPIC', '-Wall', '-Wno-unused-function',
-               '-Wno-unused-variable', '-Wno-unused-but-set-variable', '-fno-slp-vectorize']
+               '-Wno-unused-variable', '-Wno-unused-but-set-variable', '-fno-slp-vectorize',
+               # no packed fp32 arithmetic (v_pk_add / mul / fma_f32): some of its forms have given wrong results on MI355X now and then
+               '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 
 
 # per-source extra flags.  tail.hip: no fusion of a multiply and an add that the source keeps apart (the soft-argmax row arithmetic is
