@@ -34,7 +34,8 @@ extern "C" {
 
 int mpose_abi_version(void);
 /* sizeof() of the ABI structs, for binding self-checks: which = 0 geom, 1 conv operands, 2 wgrad
- * operands, 3 pack job, 4 unpack job, 5 bn job, 6 bn coef job, 7 bn_add ops, 8 reduce ops, 9 apply ops, 10 split ops, 11 sgd job. */
+ * operands, 3 pack job, 4 unpack job, 5 bn job, 6 bn coef job, 7 bn_add ops, 8 reduce ops, 9 apply ops, 10 split ops, 11 sgd job, 12 absmax ops, 13 orthogonalisation job,
+ * 14 orthogonalisation options, 15 adamw job. */
 int mpose_sizeof(int which);
 
 /* ------------------------------------------------------------------------------------------
@@ -594,6 +595,74 @@ typedef struct {
 int mpose_sgd_step(const mpose_sgd_job* jobs_dev, int n_jobs, int64_t max_n, const float* hyper_dev, void* stream);
 /* dst[0..3] = {a, b, c, d} on the stream (how the host hands the next step's hyper-parameters to a replayed graph). */
 int mpose_set4(float* dst, float a, float b, float c, float d, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Orthogonalised updates (csrc/orth.hip) and AdamW (csrc/optim.hip)
+ * ------------------------------------------------------------------------------------------ */
+/* Newton-Schulz orthogonalisation of a set of matrices of any shapes as one call:  X = G / (|G|_F + eps), then `steps` times
+ * X <- (a I + b S + c S^2) X with S = X X^T (X with its shorter axis as rows) -- the odd polynomial a s + b s^3 + c s^5 of every
+ * singular value s.  Products are three fp16 matrix-core products of two-way split operands with fp32 accumulation, for
+ * every input type; a NaN or infinite element makes its whole matrix NaN, a matrix of zeros stays zero.
+ *   jobs: a HOST array (its values travel as kernel arguments: the call can be captured and recorded);
+ *   src: row-major (rows, cols) of options.dtype (0 fp32, 1 bf16, 2 fp16), dst: the result in the same type, may be src;
+ *   buf, scale: mpose_muon_step only.  1 <= rows, cols <= 2^21, rows * cols <= 2^28 per matrix, at most 65535 matrices.
+ *   ws: mpose_orth_ws_bytes(...) bytes of device memory, 256-byte aligned, of this call alone until it has run. */
+typedef struct {
+  const void* src;
+  float* buf;
+  void* dst;
+  int32_t rows, cols;
+  float scale;
+  int32_t reserved;
+} mpose_orth_job;
+typedef struct {
+  int32_t steps;              /* 1 .. 24 */
+  int32_t dtype;
+  int32_t nesterov;
+  int32_t reserved;
+  float a, b, c;              /* refused when the polynomial lets a singular value in [0, 1] grow beyond 2^10 */
+  float eps;                  /* >= 0 */
+} mpose_orth_options;
+/* bytes of workspace, or a negative MPOSE_E* code for arguments that the calls below refuse */
+int64_t mpose_orth_ws_bytes(const mpose_orth_job* jobs, int n_jobs, const mpose_orth_options* options);
+int mpose_orthogonalize(const mpose_orth_job* jobs, int n_jobs, const mpose_orth_options* options, void* ws, int64_t ws_bytes,
+                        void* stream);
+/* One Muon step over a set of fp32 matrices: src = gradient, buf = momentum buffer, dst = parameter (all of rows * cols floats):
+ *   buf = momentum * buf + g  (first: buf = g);   u = nesterov ? g + momentum * buf : buf;
+ *   p = p * (1 - lr * weight_decay) - lr * scale * orthogonalise(u)
+ * hyper = {lr, momentum, first, weight_decay}: a HOST array, or NULL when hyper_dev, the same four floats in device memory, is
+ * given (read when the launch runs: a replayed graph or plan follows a moving schedule). */
+int mpose_muon_step(const mpose_orth_job* jobs, int n_jobs, const mpose_orth_options* options, const float* hyper,
+                    const float* hyper_dev, void* ws, int64_t ws_bytes, void* stream);
+
+/* One AdamW step over fp32 arrays (decoupled weight decay):
+ *   m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2;  p = p (1 - lr wd) - lr * c1 * m / (sqrt(v) * c2 + eps)
+ * hyper = {lr, beta1, beta2, eps, wd, c1 = 1 / (1 - beta1^t), c2 = 1 / sqrt(1 - beta2^t), 0}: HOST array, or NULL when hyper_dev (the
+ * same eight floats in device memory) is given.  jobs: a HOST array; p, g, m, v need 4-byte alignment (16 for the fast path). */
+typedef struct {
+  float* p;
+  const float* g;
+  float* m;
+  float* v;
+  int64_t n;
+} mpose_adamw_job;
+int mpose_adamw_step(const mpose_adamw_job* jobs, int n_jobs, const float* hyper, const float* hyper_dev, void* stream);
+/* dst[0..7] = src8[0..7] (src8: HOST) on the stream, by kernel arguments */
+int mpose_set8(float* dst, const float* src8, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Layer normalisation over the last axis (csrc/norm.hip):  y = (x - mean) * rstd * w + b,  rstd = 1 / sqrt(var + eps)
+ *   x, dy: `rows` rows of `cols` contiguous elements, x_ld / dy_ld elements apart; y, dx: contiguous rows.
+ *   io_dtype of x, y, dy, dx and w_dtype of w, b, dw, db: 0 fp32, 1 bf16, 2 fp16; w, b may be NULL (ones, zeros).
+ *   mean, rstd: rows floats, saved for the backward pass (forward: both may be NULL).  Statistics and sums are fp32.
+ *   dx, dw, db may be NULL (not computed).  ws: mpose_layer_norm_bwd_ws_bytes(...) bytes, needed when dw or db is given.
+ * ------------------------------------------------------------------------------------------ */
+int mpose_layer_norm_fwd(const void* x, int64_t x_ld, const void* w, const void* b, void* y, float* mean, float* rstd, int64_t rows,
+                         int cols, float eps, int io_dtype, int w_dtype, void* stream);
+int64_t mpose_layer_norm_bwd_ws_bytes(int64_t rows, int cols);
+int mpose_layer_norm_bwd(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, const void* w, const float* mean, const float* rstd,
+                         void* dx, void* dw, void* db, int64_t rows, int cols, int io_dtype, int w_dtype, void* ws, int64_t ws_bytes,
+                         void* stream);
 
 /* ------------------------------------------------------------------------------------------
  * Launch plans (csrc/plan.hip): the launches of a training iteration (reference bin/train_3d.py:154-186) recorded once and

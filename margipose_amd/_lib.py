@@ -3,6 +3,7 @@
 There is NO fallback: if the library is missing or a tensor is not a ROCm device tensor the call
 raises.  (`python -m margipose_amd.build` or `__graft_entry__.build()` compiles the library.)
 """
+import contextlib
 import ctypes
 import os
 
@@ -17,7 +18,7 @@ c_int = ctypes.c_int
 c_float = ctypes.c_float
 c_int64 = ctypes.c_int64
 
-ABI_VERSION = 16         # must equal mpose_abi_version() of the library (csrc/tail.hip)
+ABI_VERSION = 17         # must equal mpose_abi_version() of the library (csrc/tail.hip)
 MAX_GROUP = 3
 MAX_TAPS = 12
 MAX_CLASSES = 8
@@ -41,6 +42,12 @@ def lib():
         _LIB.mpose_bn_bwd_reduce_ws_bytes.restype = c_int64
         _LIB.mpose_h2_bytes.restype = c_int64
         _LIB.mpose_h2_bytes.argtypes = [c_int64, c_int]
+        _LIB.mpose_orth_ws_bytes.restype = c_int64
+        _LIB.mpose_orth_ws_bytes.argtypes = [c_void_p, c_int, c_void_p]
+        _LIB.mpose_orthogonalize.argtypes = [c_void_p, c_int, c_void_p, c_void_p, c_int64, c_void_p]
+        _LIB.mpose_muon_step.argtypes = [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]
+        _LIB.mpose_adamw_step.argtypes = [c_void_p, c_int, c_void_p, c_void_p, c_void_p]
+        _LIB.mpose_set8.argtypes = [c_void_p, c_void_p, c_void_p]
     return _LIB
 
 
@@ -113,6 +120,13 @@ def dev_f32(t, name='tensor'):
     return t
 
 
+def on_device(device):
+    """Context in which launches go to `device`'s current stream, whatever device is current outside."""
+    if torch._C._cuda_getDevice() == device.index:
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
 def ptr(t):
     return c_void_p(t.data_ptr()) if t is not None else c_void_p(None)
 
@@ -159,6 +173,11 @@ class WgradOperands(ctypes.Structure):
     _fields_ = [('in_', c_void_p), ('in_scale', c_void_p), ('in_shift', c_void_p),
                 ('gout0', c_void_p), ('gout1', c_void_p), ('dw0', c_void_p), ('dw1', c_void_p),
                 ('in_amax', c_void_p), ('gout0_amax', c_void_p), ('gout1_amax', c_void_p), ('single_product', c_int), ('planes_in', c_int)]
+
+
+class OrthOptions(ctypes.Structure):
+    _fields_ = [('steps', c_int), ('dtype', c_int), ('nesterov', c_int), ('reserved', c_int),
+                ('a', c_float), ('b', c_float), ('c', c_float), ('eps', c_float)]
 
 
 class AbsmaxOperands(ctypes.Structure):

@@ -390,6 +390,9 @@ extern "C" int mpose_sizeof(int which) {
     case 10: return (int)sizeof(mpose_split_h2_operands);
     case 11: return (int)sizeof(mpose_sgd_job);
     case 12: return (int)sizeof(mpose_absmax_operands);
+    case 13: return (int)sizeof(mpose_orth_job);
+    case 14: return (int)sizeof(mpose_orth_options);
+    case 15: return (int)sizeof(mpose_adamw_job);
     default: return -1;
   }
 }

@@ -67,3 +67,90 @@ extern "C" int mpose_sgd_step(const mpose_sgd_job* jobs_dev, int n_jobs, int64_t
   launch(sgd_step_k, dim3(dim3((unsigned)bx, (unsigned)n_jobs)), dim3(256), 0, (hipStream_t)stream, jobs_dev, hyper_dev);
   return launch_status();
 }
+
+// ---- AdamW ----
+// m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;  p = p (1 - lr wd) - lr c1 m / (sqrt(v) c2 + eps): 28 bytes per element and one pass, so
+// the rate of a large copy bounds it.  The arrays' addresses travel as kernel arguments, 96 arrays a launch (a table in device
+// memory would need an upload whenever a gradient moves, and could not be captured).
+namespace mpose {
+namespace {
+
+constexpr int kAdamJobs = 96;
+constexpr int kAdamChunk = 4096;
+struct AdamArgs {
+  mpose_adamw_job j[kAdamJobs];
+  float h[8];
+  const float* hyper_dev;
+  int n;
+};
+
+__global__ __launch_bounds__(256) void adamw_step_k(AdamArgs a) {
+  const mpose_adamw_job j = a.j[blockIdx.y];
+  const float* hp = a.hyper_dev;
+  float h[7];
+#pragma unroll
+  for (int i = 0; i < 7; ++i) h[i] = hp != nullptr ? hp[i] : a.h[i];
+  const float lr = h[0], b1 = h[1], b2 = h[2], eps = h[3], keep = 1.f - lr * h[4], step = lr * h[5], c2 = h[6];
+  auto one = [&](float& p, float g, float& m, float& v) {
+    m = fmaf(b1, m, (1.f - b1) * g);
+    v = fmaf(b2, v, (1.f - b2) * g * g);
+    p = fmaf(p, keep, -step * m / fmaf(sqrtf(v), c2, eps));
+  };
+  const bool vec = (((uintptr_t)j.p | (uintptr_t)j.g | (uintptr_t)j.m | (uintptr_t)j.v) & 15) == 0;
+  for (int64_t lo = (int64_t)blockIdx.x * kAdamChunk; lo < j.n; lo += (int64_t)gridDim.x * kAdamChunk) {
+    const int64_t hi = lo + kAdamChunk < j.n ? lo + kAdamChunk : j.n;
+    for (int q = 0; q < kAdamChunk / 1024; ++q) {
+      const int64_t i = lo + q * 1024 + threadIdx.x * 4;
+      if (vec && i + 4 <= hi) {
+        float4 p = *reinterpret_cast<float4*>(j.p + i), m = *reinterpret_cast<float4*>(j.m + i), v = *reinterpret_cast<float4*>(j.v + i);
+        const float4 g = *reinterpret_cast<const float4*>(j.g + i);
+        one(p.x, g.x, m.x, v.x); one(p.y, g.y, m.y, v.y); one(p.z, g.z, m.z, v.z); one(p.w, g.w, m.w, v.w);
+        *reinterpret_cast<float4*>(j.p + i) = p; *reinterpret_cast<float4*>(j.m + i) = m; *reinterpret_cast<float4*>(j.v + i) = v;
+      } else {
+        for (int64_t k = i; k < i + 4 && k < hi; ++k) one(j.p[k], j.g[k], j.m[k], j.v[k]);
+      }
+    }
+  }
+}
+
+struct Eight { float v[8]; };
+__global__ void set8_k(float* dst, Eight e) { if (threadIdx.x < 8) dst[threadIdx.x] = e.v[threadIdx.x]; }
+
+}  // namespace
+}  // namespace mpose
+
+extern "C" int mpose_set8(float* dst, const float* src8, void* stream) {
+  if (!dst || !src8) return MPOSE_EINVAL;
+  Eight e;
+  for (int i = 0; i < 8; ++i) e.v[i] = src8[i];
+  launch(set8_k, dim3(1), dim3(64), 0, (hipStream_t)stream, dst, e);
+  return launch_status();
+}
+
+extern "C" int mpose_adamw_step(const mpose_adamw_job* jobs, int n_jobs, const float* hyper, const float* hyper_dev, void* stream) {
+  if (n_jobs < 0 || (n_jobs > 0 && !jobs) || (!hyper && !hyper_dev)) return MPOSE_EINVAL;
+  for (int i = 0; i < n_jobs; ++i) {
+    const mpose_adamw_job& j = jobs[i];
+    if (j.n < 0 || (j.n > 0 && (!j.p || !j.g || !j.m || !j.v))) return MPOSE_EINVAL;
+    if (((uintptr_t)j.p | (uintptr_t)j.g | (uintptr_t)j.m | (uintptr_t)j.v) & 3) return MPOSE_EINVAL;
+  }
+  AdamArgs a{};
+  for (int i = 0; i < 8; ++i) a.h[i] = hyper ? hyper[i] : 0.f;
+  a.hyper_dev = hyper ? nullptr : hyper_dev;
+  for (int at = 0; at < n_jobs;) {
+    int64_t longest = 0;
+    a.n = 0;
+    while (at < n_jobs && a.n < kAdamJobs) {
+      if (jobs[at].n > 0) {
+        a.j[a.n++] = jobs[at];
+        longest = jobs[at].n > longest ? jobs[at].n : longest;
+      }
+      ++at;
+    }
+    if (a.n == 0) break;
+    int64_t bx = (longest + kAdamChunk - 1) / kAdamChunk;
+    if (bx > 1024) bx = 1024;
+    launch(adamw_step_k, dim3((unsigned)bx, (unsigned)a.n), dim3(256), 0, (hipStream_t)stream, a);
+  }
+  return launch_status();
+}

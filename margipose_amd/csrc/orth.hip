@@ -1,0 +1,746 @@
+// Newton-Schulz orthogonalisation of a set of matrices, and the Muon step built on it (gfx950).
+//
+// Mathematics.  X0 = G / (|G|_F + eps), the shorter axis (m) as rows, the longer (n) as columns; `steps` times
+//     S = X X^T,   Q = a I + b S + c S^2,   X <- Q X
+// which maps every singular value s to a s + b s^3 + c s^5.  S, Q and all products of them are polynomials in one symmetric matrix:
+// they commute, they are symmetric, and the next S is Q S Q without touching X.  So the long axis is visited twice per GROUP of steps,
+//     S = X X^T;   per step: Q = q(S), W = Q S, S <- W Q, P <- Q P;   X <- P X,
+// and every m x m product computes only the tiles on and above the diagonal (the others are their transposes).
+// In a group the rounding of S is lifted by a^2 a step where s is small: groups are as long as a^2 to the power (length - 1) stays
+// below 150 (3 + 2 steps for the customary a = 3.4445).  Relative error against float64 of one 256 x 256 matrix with
+// slowly decaying singular values, in a model of the arithmetic: one group of five 1e-4, groups of 3 + 2 and X on every step 4e-6.
+//
+// Arithmetic: like the convolutions (three fp16 products of two-way split operands, x * 2^k = h + l: 22 bits), but the scale
+// exponents come from a bound, not from a measurement: |x_ij| <= |X|_2, and a scalar recursion bounds |X|_2, |S|_2, |Q|_2 from the
+// first |X|_2 <= |G|_F / (|G|_F + eps) on (orth_scalars_k).
+//
+// Layout of a split matrix of R rows and K columns, "H8": [K / 8][plane h, l][R][8] fp16, R padded to the tile, K to 32 (zeros).  64 rows
+// of an octet are 1 KB in a row: one LDS-DMA instruction; both operands of C = A B^T are read that way, so X is kept in both
+// orientations (N: as stored, T: transposed).
+#include <math.h>
+#include "common.h"
+
+namespace mpose {
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void* lds_void_p;
+
+constexpr int kMaxSteps = 24;
+constexpr int kChunk = 4096;            // elements per workgroup of the momentum / norm pass
+constexpr int kSetupJobs = 48;          // jobs per set-up launch (they travel as kernel arguments: 4 KB)
+constexpr float kGrowth = 1024.f;       // largest singular value that a polynomial may make of one in [0, 1]
+
+struct StepExp { int x, s, q, w, p; };  // scale exponents of X (a group's first step), S, Q, W, P
+
+struct OrthJob {                        // device copy of one matrix's job
+  const void* src;
+  float* buf;
+  void* dst;
+  unsigned char *n[2], *t[2];           // X as stored / transposed (H8); two sets: a restart reads one and writes the other
+  unsigned char *s, *w, *q[2], *p[2];   // m x m (H8)
+  double* part;
+  int n_part, rows, cols, m, mp, mk;    // mp: m padded as rows, mk: m padded as the K axis
+  int rp, cp, rk, ck;                   // rows / cols padded the same two ways
+  int wide, aligned;
+  float scale, in_scale;
+  StepExp e[kMaxSteps];
+};
+
+struct OrthLayout {                     // byte offsets inside a job's part of the workspace
+  int64_t n[2], t[2], s, w, q[2], p[2], part, total;
+  int mp, mk, rp, cp, rk, ck, n_part;
+};
+
+__host__ __device__ inline int pad_to(int v, int q) { return (v + q - 1) / q * q; }
+
+__host__ __device__ inline OrthLayout orth_layout(int rows, int cols, int tile, int n_groups) {
+  OrthLayout l;
+  const int m = rows < cols ? rows : cols;
+  l.rp = pad_to(rows, tile); l.cp = pad_to(cols, tile); l.mp = pad_to(m, tile);
+  l.rk = pad_to(rows, 32); l.ck = pad_to(cols, 32); l.mk = pad_to(m, 32);
+  l.n_part = (int)(((int64_t)rows * cols + kChunk - 1) / kChunk);
+  const int64_t nb = (int64_t)l.ck * l.rp * 4, tb = (int64_t)l.rk * l.cp * 4, mb = (int64_t)l.mk * l.mp * 4;
+  int64_t at = 0;
+  for (int i = 0; i < 2; ++i) {
+    l.n[i] = at; if (i == 0 || n_groups > 1) at += nb;
+    l.t[i] = at; if (i == 0 || n_groups > 1) at += tb;
+  }
+  l.s = at; at += mb;
+  l.w = at; at += mb;
+  for (int i = 0; i < 2; ++i) { l.q[i] = at; at += mb; l.p[i] = at; at += mb; }
+  l.part = at; at += (int64_t)pad_to(l.n_part * 8, 256);
+  l.total = (at + 255) / 256 * 256;
+  return l;
+}
+
+// ---- set-up: job table and tile lists, written by the device from kernel arguments (no host memory outlives the call) ----
+struct SetupJob {
+  const void* src;
+  float* buf;
+  void* dst;
+  unsigned char* ws;
+  int rows, cols;
+  float scale;
+  int ew0, split0, sym0, fin0;          // where the job's entries start in the lists
+};
+struct SetupArgs {
+  SetupJob j[kSetupJobs];
+  OrthJob* jobs;
+  int2 *ew, *split, *sym, *fin;
+  int first, n, tile, n_groups, elem;
+};
+
+__global__ __launch_bounds__(256) void orth_setup_k(SetupArgs a) {
+  const SetupJob& j = a.j[blockIdx.x];
+  const int id = a.first + blockIdx.x;
+  const OrthLayout l = orth_layout(j.rows, j.cols, a.tile, a.n_groups);
+  if (threadIdx.x == 0) {
+    OrthJob* o = a.jobs + id;
+    o->src = j.src; o->buf = j.buf; o->dst = j.dst; o->scale = j.scale;
+    for (int i = 0; i < 2; ++i) {
+      o->n[i] = j.ws + l.n[i]; o->t[i] = j.ws + l.t[i]; o->q[i] = j.ws + l.q[i]; o->p[i] = j.ws + l.p[i];
+    }
+    o->s = j.ws + l.s; o->w = j.ws + l.w;
+    o->part = reinterpret_cast<double*>(j.ws + l.part); o->n_part = l.n_part;
+    o->rows = j.rows; o->cols = j.cols; o->m = j.rows < j.cols ? j.rows : j.cols;
+    o->mp = l.mp; o->mk = l.mk; o->rp = l.rp; o->cp = l.cp; o->rk = l.rk; o->ck = l.ck;
+    o->wide = j.rows <= j.cols;
+    const uint64_t bits = (uint64_t)j.src | (uint64_t)j.buf | (uint64_t)j.dst | ((uint64_t)j.cols * (uint64_t)a.elem);
+    o->aligned = (bits & (uint64_t)(4 * a.elem - 1)) == 0;        // four elements at a time: every row starts on that boundary
+  }
+  for (int i = threadIdx.x; i < l.n_part; i += 256) a.ew[j.ew0 + i] = make_int2(id, i);
+  const int sr = (j.rows + 63) / 64, sc = (j.cols + 63) / 64;
+  for (int i = threadIdx.x; i < sr * sc; i += 256) a.split[j.split0 + i] = make_int2(id, (i / sc) | ((i % sc) << 16));
+  const int tm = l.mp / a.tile;
+  for (int i = threadIdx.x; i < tm * tm; i += 256) {             // row-major over the upper triangle
+    const int r = i / tm, c = i % tm;
+    if (c >= r) a.sym[j.sym0 + r * tm - r * (r - 1) / 2 + (c - r)] = make_int2(id, r | (c << 16));
+  }
+  const int tr = l.rp / a.tile, tc = l.cp / a.tile;
+  for (int i = threadIdx.x; i < tr * tc; i += 256) a.fin[j.fin0 + i] = make_int2(id, (i / tc) | ((i % tc) << 16));
+}
+
+// ---- element access ----
+template <int DT>
+__device__ __forceinline__ float load1(const void* p, long i) {
+  if constexpr (DT == 0) return reinterpret_cast<const float*>(p)[i];
+  if constexpr (DT == 1) return __uint_as_float((unsigned)reinterpret_cast<const unsigned short*>(p)[i] << 16);
+  if constexpr (DT == 2) return (float)reinterpret_cast<const _Float16*>(p)[i];
+}
+template <int DT>
+__device__ __forceinline__ float4 load4(const void* p, long i) {
+  if constexpr (DT == 0) {
+    return *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i);
+  } else if constexpr (DT == 1) {
+    const uint2 v = *reinterpret_cast<const uint2*>(reinterpret_cast<const unsigned short*>(p) + i);
+    return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
+  } else {
+    const f16x4 v = *reinterpret_cast<const f16x4*>(reinterpret_cast<const _Float16*>(p) + i);
+    return make_float4((float)v[0], (float)v[1], (float)v[2], (float)v[3]);
+  }
+}
+template <int DT>
+__device__ __forceinline__ void store1(void* p, long i, float v) {
+  if constexpr (DT == 0) reinterpret_cast<float*>(p)[i] = v;
+  if constexpr (DT == 1) {             // round to nearest even; NaN stays NaN
+    const unsigned b = __float_as_uint(v);
+    reinterpret_cast<unsigned short*>(p)[i] = (v == v) ? (unsigned short)((b + 0x7fffu + ((b >> 16) & 1u)) >> 16) : (unsigned short)0x7fc0;
+  }
+  if constexpr (DT == 2) reinterpret_cast<_Float16*>(p)[i] = (_Float16)v;
+}
+
+struct Hyper { float lr, momentum, first, wd; };
+__device__ __forceinline__ Hyper get_hyper(const Hyper& h, const float* dev) {
+  return dev != nullptr ? Hyper{dev[0], dev[1], dev[2], dev[3]} : h;
+}
+
+// what is orthogonalised at one element: the input, or (MUON) the momentum update's direction
+__device__ __forceinline__ float direction(float g, float b, float mom, int nesterov) { return nesterov ? fmaf(mom, b, g) : b; }
+
+struct PassArgs {
+  const OrthJob* jobs;
+  const int2* list;
+  Hyper h;
+  const float* hyper_dev;
+  int nesterov, group;
+};
+
+// ---- pass 1: momentum update, sum of squares (float64: the squares of any finite float stay finite) ----
+template <int DT, bool MUON>
+__global__ __launch_bounds__(256) void orth_norm_k(PassArgs a) {
+  const int2 it = a.list[blockIdx.x];
+  const OrthJob& j = a.jobs[it.x];
+  const Hyper h = get_hyper(a.h, a.hyper_dev);
+  const long total = (long)j.rows * j.cols, lo = (long)it.y * kChunk, hi = lo + kChunk < total ? lo + kChunk : total;
+  const bool first = h.first != 0.f;
+  double sum = 0.0;
+  auto one = [&](float g, float& b) {
+    float u = g;
+    if constexpr (MUON) {
+      b = first ? g : fmaf(h.momentum, b, g);
+      u = direction(g, b, h.momentum, a.nesterov);
+    }
+    sum += (double)u * (double)u;
+  };
+  const bool vec = ((reinterpret_cast<uintptr_t>(j.src) & (DT == 0 ? 15 : 7)) == 0) && (!MUON || (reinterpret_cast<uintptr_t>(j.buf) & 15) == 0);
+  if (vec) {
+#pragma unroll
+    for (int q = 0; q < kChunk / 1024; ++q) {
+      const long i = lo + q * 1024 + threadIdx.x * 4;
+      if (i + 4 <= hi) {
+        const float4 g = load4<DT>(j.src, i);
+        float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (MUON && !first) b = *reinterpret_cast<const float4*>(j.buf + i);
+        one(g.x, b.x); one(g.y, b.y); one(g.z, b.z); one(g.w, b.w);
+        if (MUON) *reinterpret_cast<float4*>(j.buf + i) = b;
+      } else {
+        for (long k = i; k < hi; ++k) {
+          float b = (MUON && !first) ? j.buf[k] : 0.f;
+          one(load1<DT>(j.src, k), b);
+          if (MUON) j.buf[k] = b;
+        }
+      }
+    }
+  } else {
+    for (long k = lo + threadIdx.x; k < hi; k += 256) {
+      float b = (MUON && !first) ? j.buf[k] : 0.f;
+      one(load1<DT>(j.src, k), b);
+      if (MUON) j.buf[k] = b;
+    }
+  }
+  __shared__ double sh[4];
+  sum = wave_sum(sum);
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) j.part[it.y] = sh[0] + sh[1] + sh[2] + sh[3];
+}
+
+struct Poly { float a, b, c; };
+
+// largest |a + b t + c t^2| for t in [0, hi]
+__host__ __device__ inline float bound_q(const Poly& k, float hi) {
+  const float at_hi = fabsf(k.a + hi * (k.b + hi * k.c));
+  float r = fmaxf(fabsf(k.a), at_hi);
+  if (k.c != 0.f) {
+    const float t = -k.b / (2.f * k.c);
+    if (t > 0.f && t < hi) r = fmaxf(r, fabsf(k.a + t * (k.b + t * k.c)));
+  }
+  return r;
+}
+// largest |s (a + b s^2 + c s^4)| for s in [0, hi]: at hi or where a + 3 b t + 5 c t^2 = 0, t = s^2
+__host__ __device__ inline float bound_x(const Poly& k, float hi) {
+  auto f = [&](float t) { return sqrtf(t) * fabsf(k.a + t * (k.b + t * k.c)); };
+  const float hi2 = hi * hi;
+  float r = f(hi2);
+  if (k.c != 0.f) {
+    const float d = 9.f * k.b * k.b - 20.f * k.a * k.c;
+    if (d >= 0.f) {
+      const float root = sqrtf(d);
+      const float t0 = (-3.f * k.b - root) / (10.f * k.c), t1 = (-3.f * k.b + root) / (10.f * k.c);
+      if (t0 > 0.f && t0 < hi2) r = fmaxf(r, f(t0));
+      if (t1 > 0.f && t1 < hi2) r = fmaxf(r, f(t1));
+    }
+  } else if (k.b != 0.f) {
+    const float t = -k.a / (3.f * k.b);
+    if (t > 0.f && t < hi2) r = fmaxf(r, f(t));
+  }
+  return r;
+}
+
+// scale exponent for magnitudes up to `bound`: bound * 2^k in [2^14, 2^15).  Exponents stop at 60: magnitudes below 2^-45 (a gradient
+// that far below eps) lose relative precision step by step instead of overflowing the scale factors' product.
+__device__ __forceinline__ int exp_of(float bound) {
+  const int k = f16_scale_exp(bound * 1.01f);
+  return k > 60 ? 60 : k;
+}
+
+// ---- pass 2: one wave per matrix: |G|_F, the input scale, every step's scale exponents ----
+__global__ __launch_bounds__(64) void orth_scalars_k(OrthJob* jobs, Poly k, double eps, int steps, int group_first_mask) {
+  OrthJob& j = jobs[blockIdx.x];
+  double s = 0.0;
+  for (int i = threadIdx.x; i < j.n_part; i += 64) s += j.part[i];
+  s = wave_sum(s);
+  if (threadIdx.x != 0) return;
+  const double norm = sqrt(s), den = norm + eps;
+  float bx = norm > 0.0 ? (float)(norm / den) : 0.f, bp = 1.f;
+  StepExp e{0, 0, 0, 0, 0};
+  for (int i = 0; i < steps; ++i) {
+    const float bs = bx * bx, bq = bound_q(k, bs);
+    if ((group_first_mask >> i) & 1) { e.x = exp_of(bx); bp = 1.f; }
+    bp *= bq;
+    e.s = exp_of(bs); e.q = exp_of(bq); e.w = exp_of(bq * bs); e.p = exp_of(bp);
+    j.e[i] = e;
+    bx = bound_x(k, bx) * 1.00001f;
+  }
+  // all zeros with eps == 0: 0 / 0 stays NaN as in the formula
+  j.in_scale = (float)((double)pow2f(j.e[0].x) / den);
+}
+
+__device__ __forceinline__ void split16(float x, _Float16& h, _Float16& l) {
+  h = (_Float16)x;
+  l = (_Float16)(x - (float)h);
+}
+
+// ---- pass 3: X0 in both orientations.  One 64 x 64 tile per workgroup, transposed through LDS. ----
+template <int DT, bool MUON>
+__global__ __launch_bounds__(256) void orth_split_k(PassArgs a) {
+  const int2 it = a.list[blockIdx.x];
+  const OrthJob& j = a.jobs[it.x];
+  const int r0 = (it.y & 0xffff) * 64, c0 = (int)((unsigned)it.y >> 16) * 64;
+  const float mom = MUON ? get_hyper(a.h, a.hyper_dev).momentum : 0.f;
+  const float sc = j.in_scale;
+  const int rows = j.rows, cols = j.cols;
+  __shared__ float tile[64][65];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int r = q * 16 + (threadIdx.x >> 4), c = (threadIdx.x & 15) * 4;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (r0 + r < rows) {
+      const long i = (long)(r0 + r) * cols + c0 + c;
+      if (j.aligned && c0 + c + 4 <= cols) {
+        const float4 g = load4<DT>(j.src, i);
+        v[0] = g.x; v[1] = g.y; v[2] = g.z; v[3] = g.w;
+        if (MUON) {
+          const float4 b = *reinterpret_cast<const float4*>(j.buf + i);
+          v[0] = direction(g.x, b.x, mom, a.nesterov); v[1] = direction(g.y, b.y, mom, a.nesterov);
+          v[2] = direction(g.z, b.z, mom, a.nesterov); v[3] = direction(g.w, b.w, mom, a.nesterov);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (c0 + c + e < cols) {
+            v[e] = load1<DT>(j.src, i + e);
+            if (MUON) v[e] = direction(v[e], j.buf[i + e], mom, a.nesterov);
+          }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (c0 + c + e < cols) v[e] *= sc;             // (padding stays 0 whatever the scale is)
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) tile[r][c + e] = v[e];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const int row = threadIdx.x & 63, oct = q * 4 + (threadIdx.x >> 6);
+    f16x8 h, l;
+    if (c0 + oct * 8 < j.ck) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) { _Float16 hh, ll; split16(tile[row][oct * 8 + e], hh, ll); h[e] = hh; l[e] = ll; }
+      f16x8* d = reinterpret_cast<f16x8*>(j.n[0]) + ((long)(c0 / 8 + oct) * 2 * j.rp + r0 + row);
+      d[0] = h; d[j.rp] = l;
+    }
+    if (r0 + oct * 8 < j.rk) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) { _Float16 hh, ll; split16(tile[oct * 8 + e][row], hh, ll); h[e] = hh; l[e] = ll; }
+      f16x8* d = reinterpret_cast<f16x8*>(j.t[0]) + ((long)(r0 / 8 + oct) * 2 * j.cp + c0 + row);
+      d[0] = h; d[j.cp] = l;
+    }
+  }
+}
+
+// ---- the products ----
+// S = X X^T;  Q = q(S);  W = Q S and / or P = Q P;  S <- W Q;  X <- P X in both orientations;  the result from P X.
+// (A template argument, not a run-time value: with one kernel choosing among the symmetric products at run time hipcc 7.2 left the
+// output's address undefined on one of the paths.)
+enum { K_GRAM = 0, K_Q = 1, K_MUL = 2, K_NEXT = 3, K_X = 4, K_OUT = 5 };
+
+struct GemmArgs {
+  const OrthJob* jobs;
+  const int2* list;
+  int n_tiles;
+  int step, step0, i, parity;         // step; the group's first step; step - step0; the group's X set
+  int y0;                             // K_MUL: first of {W = Q S, P = Q P} that grid.y counts from
+  Poly k;
+  Hyper h;
+  const float* hyper_dev;
+};
+
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ f32x16 mfma(const f16x8 a, const f16x8 b, const f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+
+// Four consecutive k of one row, values v[0..3] * 2^e split into the two planes: 8 bytes each.
+__device__ __forceinline__ void put4(unsigned char* base, int rp, int row, int k, const float (&v)[4]) {
+  f16x4 h, l;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) { _Float16 hh, ll; split16(v[e], hh, ll); h[e] = hh; l[e] = ll; }
+  unsigned char* d = base + (((long)(k >> 3) * 2 * rp + row) * 16 + (k & 4) * 2);
+  *reinterpret_cast<f16x4*>(d) = h;
+  *reinterpret_cast<f16x4*>(d + (long)rp * 16) = l;
+}
+
+// C = A B^T over H8 operands, one 64 R x 64 R tile per workgroup: 2 x 2 waves, R x R accumulator blocks of 32 x 32 per wave.
+// Per k = 16: 4 R fragment reads for 3 R^2 MFMAs.  Ring of NBUF slots of k = 32, filled by LDS DMA.
+template <int R, int NBUF, int KIND, int DT>
+__global__ __launch_bounds__(256, 2) void orth_gemm_k(GemmArgs a) {
+  constexpr int T = 64 * R;
+  constexpr int kOp = 8 * T * 16, kSlot = 2 * kOp;        // bytes of one operand / both in a slot: [octet 4][plane 2][T][16 B]
+  constexpr int LW = 4 * R;                               // DMA instructions per wave and slot
+  __shared__ __attribute__((aligned(16))) unsigned char smem[NBUF * kSlot];
+  static_assert(4 * 32 * 33 * 4 <= NBUF * kSlot, "the transposing epilogue fits the ring");
+  // workgroup b runs on XCD b % 8 (observed placement, speed only): an XCD takes a contiguous run of the tile list
+  const int per = (a.n_tiles + 7) >> 3;
+  const int idx = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
+  if (idx >= a.n_tiles) return;
+  const int2 it = a.list[idx];
+  const OrthJob& j = a.jobs[it.x];
+  const int i0 = (it.y & 0xffff) * T, j0 = (int)((unsigned)it.y >> 16) * T;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int li = lane & 31, lh = lane >> 5, wm = wave & 1, wn = wave >> 1;
+
+  const StepExp e = j.e[a.step];
+  const unsigned char *A, *B;
+  unsigned char* out = nullptr;
+  int arp = j.mp, brp = j.mp, kk = j.mk, ea, eb, eo = 0;
+  if constexpr (KIND == K_GRAM) {
+    A = B = j.wide ? j.n[a.parity] : j.t[a.parity];
+    kk = j.wide ? j.ck : j.rk;
+    arp = brp = j.wide ? j.rp : j.cp;
+    ea = eb = e.x; eo = e.s; out = j.s;
+  } else if constexpr (KIND == K_Q) {
+    A = B = j.s; ea = eb = e.s; eo = e.q; out = j.q[a.i & 1];
+  } else if constexpr (KIND == K_MUL) {
+    const bool p = a.y0 + (int)blockIdx.y != 0;
+    unsigned char* const prev = a.i == 1 ? j.q[0] : j.p[(a.i + 1) & 1];
+    unsigned char* const next = j.p[a.i & 1];
+    A = j.q[a.i & 1]; ea = e.q;
+    B = p ? prev : j.s;
+    eb = p ? j.e[a.i > 0 ? a.step - 1 : a.step].p : e.s;
+    eo = p ? e.p : e.w;
+    out = p ? next : j.w;
+  } else if constexpr (KIND == K_NEXT) {
+    A = j.w; ea = e.w; B = j.q[a.i & 1]; eb = e.q; eo = j.e[a.step + 1].s; out = j.s;
+  } else {
+    const unsigned char* P = a.i == 0 ? j.q[0] : j.p[a.i & 1];
+    const unsigned char* X = j.wide ? j.t[a.parity] : j.n[a.parity];
+    A = j.wide ? P : X; B = j.wide ? X : P;
+    arp = j.rp; brp = j.cp;
+    ea = j.wide ? e.p : e.x; eb = j.wide ? e.x : e.p;
+    if (KIND == K_X) eo = j.e[a.step + 1].x;
+  }
+
+  f32x16 acc[R][R], acx[R][R];          // h x h, and the two cross products (2^-11 of it: their roundings do not matter)
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int c = 0; c < R; ++c)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) { acc[r][c][v] = 0.f; acx[r][c][v] = 0.f; }
+
+  const int n_slots = kk >> 5;
+  {
+    // waves 0, 1 fetch A, waves 2, 3 fetch B; each half of the operand's eight (octet, plane) slabs
+    const bool isb = wave >= 2;
+    const int rp = isb ? brp : arp, row0 = isb ? j0 : i0;
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(isb ? B : A), 0, (int)((unsigned)kk * (unsigned)rp * 4u), 0x00020000);
+    const unsigned slab = (unsigned)rp * 16u;
+    unsigned char* lds0 = smem + (isb ? kOp : 0) + (wave & 1) * (kOp / 2);
+    const unsigned voff = (unsigned)lane * 16u;
+    auto fetch = [&](int s) {
+      unsigned char* l = lds0 + (s % NBUF) * kSlot;
+#pragma unroll
+      for (int u = 0; u < LW; ++u) {
+        const int sl = u / R, rg = u % R;
+        const unsigned soff = ((unsigned)s * 8u + (unsigned)((wave & 1) * 4 + sl)) * slab + (unsigned)(row0 + rg * 64) * 16u;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void_p)(l + u * 1024), 16, (int)voff, (int)soff, 0, 0);
+      }
+    };
+#pragma unroll
+    for (int s = 0; s < NBUF - 1; ++s)
+      if (s < n_slots) fetch(s);
+    for (int s = 0; s < n_slots; ++s) {
+      if (s + NBUF - 2 < n_slots) wait_vm<LW * (NBUF - 2)>();
+      else wait_vm<0>();
+      __builtin_amdgcn_s_waitcnt(0xC07F);          // lgkmcnt(0): this wave's reads of slot s - 1 are in registers
+      __builtin_amdgcn_s_barrier();                // slot s is whole, slot s - 1 is free
+      asm volatile("" ::: "memory");
+      if (s + NBUF - 1 < n_slots) fetch(s + NBUF - 1);
+      const unsigned char* pa = smem + (s % NBUF) * kSlot + (wm * 32 * R + li) * 16;
+      const unsigned char* pb = smem + (s % NBUF) * kSlot + kOp + (wn * 32 * R + li) * 16;
+#pragma unroll
+      for (int k16 = 0; k16 < 2; ++k16) {
+        f16x8 ah[R], al[R], bh[R], bl[R];
+        const int o = (k16 * 2 + lh) * 2 * T * 16;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          ah[r] = *reinterpret_cast<const f16x8*>(pa + o + r * 512);
+          bh[r] = *reinterpret_cast<const f16x8*>(pb + o + r * 512);
+          al[r] = *reinterpret_cast<const f16x8*>(pa + o + T * 16 + r * 512);
+          bl[r] = *reinterpret_cast<const f16x8*>(pb + o + T * 16 + r * 512);
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int c = 0; c < R; ++c) {
+            acc[r][c] = mfma(ah[r], bh[c], acc[r][c]);
+            acx[r][c] = mfma(ah[r], bl[c], acx[r][c]);
+            acx[r][c] = mfma(al[r], bh[c], acx[r][c]);
+          }
+      }
+    }
+  }
+
+  // Accumulator block: lane (li, lh) holds column li, rows 8 g + 4 lh + v (g, v = 0..3).
+  const float da = pow2f(-ea), db = pow2f(-eb), so = pow2f(eo);
+  const int ib = i0 + wm * 32 * R, jb = j0 + wn * 32 * R;
+  if constexpr (KIND == K_OUT) {
+    const Hyper h = get_hyper(a.h, a.hyper_dev);
+    const float keep = 1.f - h.lr * h.wd, rate = h.lr * j.scale;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int c = 0; c < R; ++c) {
+        const int col = jb + c * 32 + li;
+        if (col >= j.cols) continue;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const int row = ib + r * 32 + 8 * (v >> 2) + 4 * lh + (v & 3);
+          if (row >= j.rows) continue;
+          const float x = (acc[r][c][v] + acx[r][c][v]) * da * db;
+          const long o = (long)row * j.cols + col;
+          if constexpr (DT == 3) {
+            float* p = reinterpret_cast<float*>(j.dst) + o;
+            *p = fmaf(-rate, x, *p * keep);
+          } else {
+            store1<DT>(j.dst, o, x);
+          }
+        }
+      }
+    return;
+  } else {
+    // where the tile goes: rows of the first layout = C's columns, its K axis = C's rows; the second layout the other way round
+    unsigned char* d1 = out;
+    unsigned char* d2 = out;
+    int rp1 = j.mp, rp2 = j.mp, lim1 = j.m, lim2 = j.m, k1 = j.mk, k2 = j.mk;
+    if constexpr (KIND == K_X) {
+      d1 = j.t[a.parity ^ 1]; rp1 = j.cp; lim1 = j.rows; k1 = j.rk;
+      d2 = j.n[a.parity ^ 1]; rp2 = j.rp; lim2 = j.cols; k2 = j.ck;
+    }
+    const bool second = KIND == K_X || i0 != j0;      // (a diagonal tile holds both halves itself)
+    __syncthreads();                                   // the ring becomes the transposing buffer
+    float* tr = reinterpret_cast<float*>(smem) + wave * 32 * 33;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int c = 0; c < R; ++c) {
+        const int col = jb + c * 32 + li;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int k = ib + r * 32 + 8 * g + 4 * lh;
+          float x[4];
+#pragma unroll
+          for (int v = 0; v < 4; ++v) x[v] = (acc[r][c][4 * g + v] + acx[r][c][4 * g + v]) * da * db;
+          if constexpr (KIND == K_Q) {
+            if (k < j.mk) {
+              const unsigned char* sp = j.s + (((long)(k >> 3) * 2 * j.mp + col) * 16 + (k & 4) * 2);
+              const f16x4 sh = *reinterpret_cast<const f16x4*>(sp), sl = *reinterpret_cast<const f16x4*>(sp + (long)j.mp * 16);
+#pragma unroll
+              for (int v = 0; v < 4; ++v) {
+                const float s = ((float)sh[v] + (float)sl[v]) * da;
+                x[v] = fmaf(a.k.c, x[v], a.k.b * s) + (k + v == col ? a.k.a : 0.f);
+              }
+            }
+          }
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            x[v] *= so;
+            tr[(8 * g + 4 * lh + v) * 33 + li] = x[v];
+            if (k + v >= lim1) x[v] = 0.f;
+          }
+          if (k < k1) put4(d1, rp1, col, k, x);
+        }
+        if (second) {
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // (one wave: its LDS accesses execute in order)
+          const int row = ib + r * 32 + li;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const int k = jb + c * 32 + 8 * g + 4 * lh;
+            float x[4];
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+              x[v] = tr[li * 33 + 8 * g + 4 * lh + v];
+              if (k + v >= lim2) x[v] = 0.f;
+            }
+            if (k < k2) put4(d2, rp2, row, k, x);
+          }
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
+      }
+  }
+}
+
+// ---- host ----
+struct Groups { int n, first[kMaxSteps], size[kMaxSteps], mask; };
+
+Groups make_groups(int steps, float a) {
+  const double a2 = (double)a * a;
+  int longest = 1;
+  for (double lift = a2; lift <= 150.0 && longest < steps; lift *= a2 > 1.0 ? a2 : 1.0) ++longest;
+  Groups g{};
+  g.n = (steps + longest - 1) / longest;
+  int at = 0;
+  for (int i = 0; i < g.n; ++i) {
+    g.first[i] = at;
+    g.size[i] = (steps - at + (g.n - i) - 1) / (g.n - i);        // as even as possible, the longer ones first
+    g.mask |= 1 << at;
+    at += g.size[i];
+  }
+  return g;
+}
+
+struct OrthPlan {
+  int64_t jobs_b, ew_b, split_b, sym_b, fin_b, head_b, total_b;
+  int64_t n_ew, n_split, n_sym, n_fin;
+  int tile;
+  Groups g;
+};
+
+int make_plan(const mpose_orth_job* jobs, int n_jobs, const mpose_orth_options* o, OrthPlan& p) {
+  if (n_jobs < 0 || n_jobs > 65535 || !o || (n_jobs > 0 && !jobs)) return MPOSE_EINVAL;
+  if (o->steps < 1 || o->steps > kMaxSteps || o->dtype < 0 || o->dtype > 2 || !(o->eps >= 0.f) || !isfinite(o->eps)) return MPOSE_EINVAL;
+  if (!isfinite(o->a) || !isfinite(o->b) || !isfinite(o->c)) return MPOSE_EINVAL;
+  const Poly k{o->a, o->b, o->c};
+  float bx = 1.f;
+  for (int i = 0; i < o->steps; ++i) {
+    if (!(bound_q(k, bx * bx) <= kGrowth)) return MPOSE_EINVAL;
+    bx = bound_x(k, bx);
+    if (!(bx <= kGrowth)) return MPOSE_EINVAL;
+  }
+  p = OrthPlan{};
+  p.g = make_groups(o->steps, o->a);
+  p.tile = 64;
+  int64_t body = 0;
+  for (int i = 0; i < n_jobs; ++i) {
+    const int rows = jobs[i].rows, cols = jobs[i].cols;
+    if (rows < 1 || cols < 1 || rows > (1 << 21) || cols > (1 << 21) || (int64_t)rows * cols > (1 << 28)) return MPOSE_EINVAL;
+    const OrthLayout l = orth_layout(rows, cols, p.tile, p.g.n);
+    body += l.total;
+    p.n_ew += l.n_part;
+    p.n_split += (int64_t)((rows + 63) / 64) * ((cols + 63) / 64);
+    const int64_t tm = l.mp / p.tile;
+    p.n_sym += tm * (tm + 1) / 2;
+    p.n_fin += (int64_t)(l.rp / p.tile) * (l.cp / p.tile);
+  }
+  if (p.n_ew > (1 << 30) || p.n_split > (1 << 30) || p.n_sym > (1 << 30) || p.n_fin > (1 << 30)) return MPOSE_EINVAL;
+  auto up = [](int64_t b) { return (b + 255) / 256 * 256; };
+  p.jobs_b = up((int64_t)n_jobs * (int64_t)sizeof(OrthJob));
+  p.ew_b = up(p.n_ew * 8); p.split_b = up(p.n_split * 8); p.sym_b = up(p.n_sym * 8); p.fin_b = up(p.n_fin * 8);
+  p.head_b = p.jobs_b + p.ew_b + p.split_b + p.sym_b + p.fin_b;
+  p.total_b = p.head_b + body;
+  return 0;
+}
+
+template <int KIND, int DT = 0>
+void gemm(const GemmArgs& a, int ny, hipStream_t s) {
+  launch(orth_gemm_k<1, 3, KIND, DT>, dim3((unsigned)((a.n_tiles + 7) / 8 * 8), (unsigned)ny), dim3(256), 0, s, a);
+}
+
+int run(const mpose_orth_job* jobs, int n_jobs, const mpose_orth_options* o, bool muon, const Hyper& h, const float* hyper_dev, void* ws, int64_t ws_bytes,
+        hipStream_t s) {
+  OrthPlan p;
+  const int rc = make_plan(jobs, n_jobs, o, p);
+  if (rc != 0) return rc;
+  if (n_jobs == 0) return 0;
+  if (!ws || ((uintptr_t)ws & 255) || ws_bytes < p.total_b) return MPOSE_EINVAL;
+  const int elem = o->dtype == 0 ? 4 : 2;
+  for (int i = 0; i < n_jobs; ++i) {
+    if (!jobs[i].src || !jobs[i].dst || (muon && !jobs[i].buf)) return MPOSE_EINVAL;
+    if (((uintptr_t)jobs[i].src | (uintptr_t)jobs[i].dst) & (uintptr_t)(elem - 1)) return MPOSE_EINVAL;
+    if (muon && ((uintptr_t)jobs[i].buf & 3)) return MPOSE_EINVAL;
+  }
+  unsigned char* base = (unsigned char*)ws;
+  SetupArgs sa{};
+  sa.jobs = (OrthJob*)base; base += p.jobs_b;
+  sa.ew = (int2*)base; base += p.ew_b;
+  sa.split = (int2*)base; base += p.split_b;
+  sa.sym = (int2*)base; base += p.sym_b;
+  sa.fin = (int2*)base; base += p.fin_b;
+  sa.tile = p.tile; sa.n_groups = p.g.n; sa.elem = elem;
+  int ew = 0, split = 0, sym = 0, fin = 0;
+  for (int i = 0; i < n_jobs; ++i) {
+    if (sa.n == 0) sa.first = i;
+    SetupJob& j = sa.j[sa.n++];
+    j = SetupJob{jobs[i].src, muon ? jobs[i].buf : nullptr, jobs[i].dst, base, jobs[i].rows, jobs[i].cols, jobs[i].scale, ew, split, sym, fin};
+    const OrthLayout l = orth_layout(j.rows, j.cols, p.tile, p.g.n);
+    base += l.total;
+    ew += l.n_part;
+    split += ((j.rows + 63) / 64) * ((j.cols + 63) / 64);
+    const int tm = l.mp / p.tile;
+    sym += tm * (tm + 1) / 2;
+    fin += (l.rp / p.tile) * (l.cp / p.tile);
+    if (sa.n == kSetupJobs || i == n_jobs - 1) {
+      launch(orth_setup_k, dim3((unsigned)sa.n), dim3(256), 0, s, sa);
+      sa.n = 0;
+    }
+  }
+  PassArgs pa{};
+  pa.jobs = sa.jobs; pa.h = h; pa.hyper_dev = hyper_dev; pa.nesterov = o->nesterov;
+  const Poly k{o->a, o->b, o->c};
+  pa.list = sa.ew;
+  const dim3 ge((unsigned)p.n_ew), gs((unsigned)p.n_split), wg(256);
+  if (muon) launch(orth_norm_k<0, true>, ge, wg, 0, s, pa);
+  else if (o->dtype == 0) launch(orth_norm_k<0, false>, ge, wg, 0, s, pa);
+  else if (o->dtype == 1) launch(orth_norm_k<1, false>, ge, wg, 0, s, pa);
+  else launch(orth_norm_k<2, false>, ge, wg, 0, s, pa);
+  launch(orth_scalars_k, dim3((unsigned)n_jobs), dim3(64), 0, s, sa.jobs, k, (double)o->eps, o->steps, p.g.mask);
+  pa.list = sa.split;
+  if (muon) launch(orth_split_k<0, true>, gs, wg, 0, s, pa);
+  else if (o->dtype == 0) launch(orth_split_k<0, false>, gs, wg, 0, s, pa);
+  else if (o->dtype == 1) launch(orth_split_k<1, false>, gs, wg, 0, s, pa);
+  else launch(orth_split_k<2, false>, gs, wg, 0, s, pa);
+
+  GemmArgs ga{};
+  ga.jobs = sa.jobs; ga.k = k; ga.h = h; ga.hyper_dev = hyper_dev;
+  for (int g = 0; g < p.g.n; ++g) {
+    ga.step0 = p.g.first[g]; ga.parity = g & 1;
+    ga.list = sa.sym; ga.n_tiles = (int)p.n_sym;
+    ga.step = ga.step0; ga.i = 0;
+    gemm<K_GRAM>(ga, 1, s);
+    for (int i = 0; i < p.g.size[g]; ++i) {
+      ga.i = i; ga.step = ga.step0 + i;
+      const bool last = i == p.g.size[g] - 1;
+      gemm<K_Q>(ga, 1, s);
+      // W = Q S unless this is the group's last step, P = Q P unless it is its first
+      ga.y0 = last ? 1 : 0;
+      if (!last || i > 0) gemm<K_MUL>(ga, (last ? 0 : 1) + (i > 0 ? 1 : 0), s);
+      if (!last) gemm<K_NEXT>(ga, 1, s);
+    }
+    ga.list = sa.fin; ga.n_tiles = (int)p.n_fin;
+    if (g + 1 < p.g.n) gemm<K_X>(ga, 1, s);
+    else if (muon) gemm<K_OUT, 3>(ga, 1, s);
+    else if (o->dtype == 0) gemm<K_OUT, 0>(ga, 1, s);
+    else if (o->dtype == 1) gemm<K_OUT, 1>(ga, 1, s);
+    else gemm<K_OUT, 2>(ga, 1, s);
+  }
+  return launch_status();
+}
+
+}  // namespace
+}  // namespace mpose
+
+using namespace mpose;
+
+extern "C" int64_t mpose_orth_ws_bytes(const mpose_orth_job* jobs, int n_jobs, const mpose_orth_options* options) {
+  OrthPlan p;
+  const int rc = make_plan(jobs, n_jobs, options, p);
+  return rc != 0 ? (int64_t)rc : p.total_b;
+}
+
+extern "C" int mpose_orthogonalize(const mpose_orth_job* jobs, int n_jobs, const mpose_orth_options* options, void* ws, int64_t ws_bytes, void* stream) {
+  return run(jobs, n_jobs, options, false, Hyper{0.f, 0.f, 0.f, 0.f}, nullptr, ws, ws_bytes, (hipStream_t)stream);
+}
+
+extern "C" int mpose_muon_step(const mpose_orth_job* jobs, int n_jobs, const mpose_orth_options* options, const float* hyper, const float* hyper_dev, void* ws,
+                               int64_t ws_bytes, void* stream) {
+  if ((!hyper && !hyper_dev) || (options && options->dtype != 0)) return MPOSE_EINVAL;
+  const Hyper h = hyper ? Hyper{hyper[0], hyper[1], hyper[2], hyper[3]} : Hyper{0.f, 0.f, 0.f, 0.f};
+  return run(jobs, n_jobs, options, true, h, hyper ? nullptr : hyper_dev, ws, ws_bytes, (hipStream_t)stream);
+}

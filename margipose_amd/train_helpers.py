@@ -3,6 +3,7 @@
 per-step sequence  scheduler.batch_step -> model(x) -> forward_loss -> zero_grad -> backward -> optimiser.step
 can be driven exactly like the reference drives it.  No dataset / telemetry code (out of scope)."""
 import bisect
+import math
 
 import torch
 
@@ -267,6 +268,290 @@ class DeviceSGD:
             g.update(s)
 
 
+IO_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+MUON_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+_ORTH_JOB_DT = [('src', 'u8'), ('buf', 'u8'), ('dst', 'u8'), ('rows', 'i4'), ('cols', 'i4'), ('scale', 'f4'), ('reserved', 'i4')]
+_ADAMW_JOB_DT = [('p', 'u8'), ('g', 'u8'), ('m', 'u8'), ('v', 'u8'), ('n', 'i8')]
+
+
+def _jobs(n, fields, struct):
+    """A host job array of the C ABI, checked against the library's struct."""
+    import numpy as np
+    dt = np.dtype(fields)
+    if _lib.lib().mpose_sizeof(struct) != dt.itemsize:
+        raise _lib.MposeError('ABI struct %d: library and binding disagree' % struct)
+    return np.zeros(n, dtype=dt)
+
+
+def _pointers(tensors):
+    import numpy as np
+    return np.fromiter(map(torch.Tensor.data_ptr, tensors), dtype=np.uint64, count=len(tensors))
+
+
+def _orth_options(steps, coefficients, eps, dtype, nesterov=False):
+    try:
+        a, b, c = (float(v) for v in coefficients)
+    except (TypeError, ValueError):
+        raise _lib.MposeError('Newton-Schulz coefficients are three numbers (a, b, c), got %r' % (coefficients,))
+    return _lib.OrthOptions(int(steps), IO_DTYPES[dtype], int(bool(nesterov)), 0, a, b, c, float(eps))
+
+
+def _orth_workspace_bytes(jobs, options):
+    import ctypes
+    n = _lib.lib().mpose_orth_ws_bytes(jobs.ctypes.data, len(jobs), ctypes.addressof(options))
+    if n < 0:
+        raise _lib.MposeError('Newton-Schulz: refused (code %d): 1..24 steps, eps >= 0, a polynomial that keeps singular values of [0, 1] below 2^10, '
+                              'matrices of at most 2^28 elements with axes of at most 2^21' % n)
+    return n
+
+
+def orthogonalize(matrices, steps=5, coefficients=MUON_COEFFICIENTS, eps=1e-7):
+    """Newton-Schulz orthogonalisation (csrc/orth.hip): every matrix G becomes X after X = G / (|G|_F + eps) and `steps` times
+    X <- (a I + b S + c S^2) X, S = X X^T -- near U V^T of G = U diag(s) V^T.  `matrices`: a tensor or a list of tensors of any shapes,
+    float32, bfloat16 or float16 (one type and device per call); a tensor of more than two dimensions is the matrix of its first
+    axis against the rest, like a convolution's weight.  Returns new tensors of the same shapes and type; the arithmetic is
+    float32-equivalent for every type.  Not differentiable.  All matrices of a call share its launches: pass them together."""
+    import ctypes
+    single = isinstance(matrices, torch.Tensor)
+    mats = [matrices] if single else list(matrices)
+    if not mats:
+        return []
+    first = mats[0]
+    for t in mats:
+        if not isinstance(t, torch.Tensor) or t.dim() < 2:
+            raise _lib.MposeError('orthogonalize needs tensors of at least two dimensions')
+        if not t.is_cuda:
+            raise _lib.MposeError('orthogonalize: matrices must live on a ROCm device (got %s): margipose_amd has no CPU path' % t.device)
+        if t.dtype != first.dtype or t.device != first.device or t.dtype not in IO_DTYPES:
+            raise _lib.MposeError('orthogonalize: matrices must share one device and one of float32, bfloat16, float16')
+        if t.requires_grad and torch.is_grad_enabled():
+            raise _lib.MposeError('orthogonalize is not differentiable: pass detached tensors or call it under torch.no_grad()')
+    options = _orth_options(steps, coefficients, eps, first.dtype)
+    with _lib.on_device(first.device), torch.no_grad():
+        if _lib.plan_recording() and not all(t.is_contiguous() for t in mats):
+            raise _lib.MposeError('orthogonalize: matrices must be contiguous while a launch plan is recorded')
+        srcs = [t.contiguous() for t in mats]
+        outs = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in srcs]
+        work = [(s, o) for s, o in zip(srcs, outs) if s.numel()]
+        jobs = _jobs(len(work), _ORTH_JOB_DT, 13)
+        for k, (s, o) in enumerate(work):
+            jobs[k] = (s.data_ptr(), 0, o.data_ptr(), s.shape[0], s.numel() // s.shape[0], 1.0, 0)
+        n = _orth_workspace_bytes(jobs, options)
+        if work:
+            ws = torch.empty(n, dtype=torch.uint8, device=first.device)
+            _lib.check(_lib.lib().mpose_orthogonalize(jobs.ctypes.data, len(jobs), ctypes.addressof(options), ws.data_ptr(), n, _lib.stream_ptr()),
+                       'mpose_orthogonalize')
+    return outs[0] if single else outs
+
+
+class _DeviceStep:
+    """What DeviceAdamW and DeviceMuon share with DeviceSGD's protocol: hyper-parameters travel as kernel arguments in an eager step
+    and live in device memory inside a captured graph or a launch plan, where before_replay() refreshes them."""
+
+    def _check_params(self, params, who):
+        if not all(isinstance(p, torch.Tensor) and p.is_cuda and p.dtype == torch.float32 for p in params):
+            raise _lib.MposeError('%s needs float32 parameters on a ROCm device' % who)
+        if not all(p.is_contiguous() for p in params):
+            raise _lib.MposeError('%s needs contiguous parameters' % who)
+        if len(set(map(id, params))) != len(params) or len({p.device for p in params}) > 1:
+            raise _lib.MposeError('%s needs each parameter once, and all on one device' % who)
+
+    def _arena(self, params, device):
+        """One zeroed arena with a 16-byte aligned place for each parameter; (arena, the places' addresses)."""
+        import numpy as np
+        sizes = np.array([(p.numel() + 3) // 4 * 4 for p in params], dtype=np.int64)
+        offsets = np.concatenate([[0], np.cumsum(sizes)]) if len(sizes) else np.zeros(1, np.int64)
+        arena = torch.zeros(int(offsets[-1]), dtype=torch.float32, device=device)
+        return arena, (np.uint64(arena.data_ptr()) + 4 * offsets[:-1].astype(np.uint64)).astype(np.uint64)
+
+    def _gather(self, params, known, who):
+        """Addresses of the gradients and the parameters; parameters that moved since the last step are checked again."""
+        grads = [p.grad for p in params]
+        if any(g is None for g in grads):
+            raise RuntimeError('%s.step(): a parameter has no gradient' % who)
+        if not all(map(torch.Tensor.is_contiguous, grads)):
+            raise RuntimeError('%s needs contiguous gradients' % who)
+        at = _pointers(params)
+        if known is None or (at != known).any():
+            self._check_params(params, who)
+        return _pointers(grads), at
+
+    def zero_grad(self, set_to_none=True):
+        for group in self.param_groups:
+            for p in group['params']:
+                if set_to_none:
+                    p.grad = None
+                elif p.grad is not None:
+                    p.grad.zero_()
+
+    def _recorded(self):
+        return torch.cuda.is_current_stream_capturing() or _lib.plan_recording()
+
+    def before_replay(self):
+        self.upload_hyper()
+        self.steps += 1
+        torch.autograd.graph.increment_version([p for g in self.param_groups for p in g['params']])
+
+
+class DeviceAdamW(_DeviceStep):
+    """torch.optim.AdamW's update (decoupled weight decay, no amsgrad) over all parameters as launches of csrc/optim.hip, 96 arrays
+    each:  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2;  p = p (1 - lr wd) - lr m^ / (sqrt(v^) + eps).
+    Duck-types DeviceSGD: works in training_step, GraphedTrainStep and PlannedTrainStep, and under make_1cycle -- the schedule's
+    `momentum` is beta1.  The moments are two flat arenas (exp_avg_arena, exp_avg_sq_arena), a parameter every 16 bytes."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01):
+        params = list(params)
+        if not params:
+            raise _lib.MposeError('DeviceAdamW needs at least one parameter')
+        self._check_params(params, 'DeviceAdamW')
+        b1, b2 = (float(b) for b in betas)
+        if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and eps >= 0.0 and lr >= 0.0 and weight_decay >= 0.0):
+            raise _lib.MposeError('DeviceAdamW needs 0 <= betas < 1, and lr, eps and weight_decay that are not negative')
+        self.params = params
+        self.param_groups = [{'params': params, 'lr': float(lr), 'momentum': b1, 'beta2': b2, 'eps': float(eps), 'weight_decay': float(weight_decay)}]
+        dev = params[0].device
+        self.exp_avg_arena, m = self._arena(params, dev)
+        self.exp_avg_sq_arena, v = self._arena(params, dev)
+        self._table = _jobs(len(params), _ADAMW_JOB_DT, 15)
+        self._table['m'], self._table['v'], self._table['n'] = m, v, [p.numel() for p in params]
+        self._known = None
+        self._hyper = torch.zeros(8, dtype=torch.float32, device=dev)
+        self.steps = 0
+
+    def _hyper_values(self):
+        import numpy as np
+        g, t = self.param_groups[0], self.steps + 1
+        return np.array([g['lr'], g['momentum'], g['beta2'], g['eps'], g['weight_decay'], 1.0 / (1.0 - g['momentum'] ** t),
+                         1.0 / math.sqrt(1.0 - g['beta2'] ** t), 0.0], dtype=np.float32)
+
+    def upload_hyper(self):
+        """Hand the next step's hyper-parameters to a captured or recorded step (values travel as kernel arguments)."""
+        with _lib.on_device(self._hyper.device):
+            _lib.check(_lib.lib().mpose_set8(self._hyper.data_ptr(), self._hyper_values().ctypes.data, _lib.stream_ptr()), 'mpose_set8')
+
+    def _launch(self, recorded):
+        self._table['g'], self._table['p'] = g, p = self._gather(self.params, self._known, 'DeviceAdamW')
+        self._known = p
+        hyper = None if recorded else self._hyper_values()
+        _lib.check(_lib.lib().mpose_adamw_step(self._table.ctypes.data, len(self._table), hyper.ctypes.data if hyper is not None else None,
+                                               self._hyper.data_ptr(), _lib.stream_ptr()), 'mpose_adamw_step')
+
+    def step(self):
+        with _lib.on_device(self._hyper.device):
+            self._launch(self._recorded())
+        if not torch.cuda.is_current_stream_capturing():
+            self.steps += 1
+            torch.autograd.graph.increment_version(self.params)       # (the kernels write the parameters behind autograd's back)
+
+    def state_dict(self):
+        return {'state': {'exp_avg': self.exp_avg_arena.detach().cpu(), 'exp_avg_sq': self.exp_avg_sq_arena.detach().cpu(), 'steps': self.steps},
+                'param_groups': [{k: v for k, v in g.items() if k != 'params'} for g in self.param_groups]}
+
+    def load_state_dict(self, sd):
+        self.exp_avg_arena.copy_(sd['state']['exp_avg'])
+        self.exp_avg_sq_arena.copy_(sd['state']['exp_avg_sq'])
+        self.steps = int(sd['state']['steps'])
+        for g, s in zip(self.param_groups, sd['param_groups']):
+            g.update(s)
+
+
+class DeviceMuon(_DeviceStep):
+    """Muon: momentum, then an orthogonalised update for every weight matrix -- all matrices of the model in the same few launches
+    (csrc/orth.hip) -- and AdamW for the parameters of fewer than two dimensions and for `vectors`:
+        buf = momentum buf + g;   u = g + momentum buf (nesterov) or buf;   p = p (1 - lr wd) - lr * 0.2 sqrt(max(rows, cols)) orthogonalize(u)
+    A weight of more than two dimensions is the matrix of its first axis against the rest.  The factor gives the update the size of an
+    AdamW update, so that ONE learning rate and one 1cycle schedule (make_1cycle) drive both parts; `vector_options` overrides
+    DeviceAdamW's arguments.  Duck-types DeviceSGD: training_step, GraphedTrainStep and PlannedTrainStep take it.  The momentum buffers are one flat
+    arena (momentum_arena, a matrix every 16 bytes, in the order of param_groups[0]['params'])."""
+
+    def __init__(self, params, lr=0.02, momentum=0.95, weight_decay=0.0, nesterov=True, ns_steps=5, ns_coefficients=MUON_COEFFICIENTS, ns_eps=1e-7,
+                 vectors=(), vector_options=None):
+        params = list(params)
+        matrices = [p for p in params if p.dim() >= 2]
+        vectors = [p for p in params if p.dim() < 2] + list(vectors)
+        if not matrices:
+            raise _lib.MposeError('DeviceMuon needs at least one parameter of two dimensions or more')
+        self._check_params(matrices + vectors, 'DeviceMuon')
+        if not (0.0 <= momentum < 1.0 and lr >= 0.0 and weight_decay >= 0.0):
+            raise _lib.MposeError('DeviceMuon needs 0 <= momentum < 1, and lr and weight_decay that are not negative')
+        self.matrices = [p for p in matrices if p.numel()]
+        self._options = _orth_options(ns_steps, ns_coefficients, ns_eps, torch.float32, nesterov)
+        dev = matrices[0].device
+        self.momentum_arena, bufs = self._arena(self.matrices, dev)
+        self._table = _jobs(len(self.matrices), _ORTH_JOB_DT, 13)
+        shapes = [(p.shape[0], p.numel() // p.shape[0]) for p in self.matrices]
+        self._table['buf'] = bufs
+        self._table['rows'], self._table['cols'] = [s[0] for s in shapes], [s[1] for s in shapes]
+        self._table['scale'] = [0.2 * math.sqrt(max(s)) for s in shapes]
+        self._ws_bytes = _orth_workspace_bytes(self._table, self._options)
+        self._known = None
+        self._hyper = torch.zeros(4, dtype=torch.float32, device=dev)
+        self.param_groups = [{'params': self.matrices, 'lr': float(lr), 'momentum': float(momentum), 'weight_decay': float(weight_decay)}]
+        self.vector_optimiser = None
+        self.exp_avg_arena = self.exp_avg_sq_arena = torch.zeros(0, dtype=torch.float32, device=dev)
+        if vectors:
+            self.vector_optimiser = DeviceAdamW(vectors, **dict({'lr': lr}, **(vector_options or {})))
+            self.param_groups += self.vector_optimiser.param_groups
+            self.exp_avg_arena, self.exp_avg_sq_arena = self.vector_optimiser.exp_avg_arena, self.vector_optimiser.exp_avg_sq_arena
+        self._all = self.matrices + vectors
+        self.steps = 0
+
+    @property
+    def steps(self):
+        return self._steps
+
+    @steps.setter
+    def steps(self, n):
+        self._steps = n
+        if self.vector_optimiser is not None:
+            self.vector_optimiser.steps = n
+
+    def _hyper_values(self):
+        import numpy as np
+        g = self.param_groups[0]
+        return np.array([g['lr'], g['momentum'], 1.0 if self._steps == 0 else 0.0, g['weight_decay']], dtype=np.float32)
+
+    def upload_hyper(self):
+        """Hand the next step's hyper-parameters to a captured or recorded step (values travel as kernel arguments)."""
+        f = _lib.c_float
+        with _lib.on_device(self._hyper.device):
+            _lib.check(_lib.lib().mpose_set4(_lib.ptr(self._hyper), *[f(float(v)) for v in self._hyper_values()], _lib.stream_ptr()), 'mpose_set4')
+            if self.vector_optimiser is not None:
+                self.vector_optimiser.upload_hyper()
+
+    def step(self):
+        import ctypes
+        with _lib.on_device(self._hyper.device):
+            recorded = self._recorded()
+            self._table['src'], self._table['dst'] = g, p = self._gather(self.matrices, self._known, 'DeviceMuon')
+            self._known = p
+            hyper = None if recorded else self._hyper_values()
+            # (scratch of this step alone, from the allocator: a captured graph or a recorded plan keeps its own)
+            ws = torch.empty(self._ws_bytes, dtype=torch.uint8, device=self._hyper.device)
+            _lib.check(_lib.lib().mpose_muon_step(self._table.ctypes.data, len(self._table), ctypes.addressof(self._options),
+                                                  hyper.ctypes.data if hyper is not None else None, self._hyper.data_ptr(), ws.data_ptr(), self._ws_bytes,
+                                                  _lib.stream_ptr()), 'mpose_muon_step')
+            if self.vector_optimiser is not None:
+                self.vector_optimiser._launch(recorded)
+        if not torch.cuda.is_current_stream_capturing():
+            self.steps += 1
+            torch.autograd.graph.increment_version(self._all)         # (the kernels write the parameters behind autograd's back)
+
+    def state_dict(self):
+        state = {'momentum_buffers': self.momentum_arena.detach().cpu(), 'steps': self.steps}
+        if self.vector_optimiser is not None:
+            state['vectors'] = self.vector_optimiser.state_dict()['state']
+        return {'state': state, 'param_groups': [{k: v for k, v in g.items() if k != 'params'} for g in self.param_groups]}
+
+    def load_state_dict(self, sd):
+        self.momentum_arena.copy_(sd['state']['momentum_buffers'])
+        if self.vector_optimiser is not None:
+            self.vector_optimiser.load_state_dict({'state': sd['state']['vectors'], 'param_groups': []})
+        self.steps = int(sd['state']['steps'])
+        for g, s in zip(self.param_groups, sd['param_groups']):
+            g.update(s)
+
+
 class GraphedTrainStep:
     """One training iteration of the reference (bin/train_3d.py:154-186: model(x) -> forward_loss -> zero_grad -> backward ->
     optimiser.step) captured ONCE as a HIP graph and replayed: every buffer of a step has a fixed address (engine.py: arenas,
@@ -275,7 +560,7 @@ class GraphedTrainStep:
         step = GraphedTrainStep(model, optimiser, x, target, mask)          # example tensors fix the shapes
         out, loss = step(x, target, mask)                                    # copies the batch in, replays
 
-    `optimiser`: DeviceSGD (hyper-parameters may change every step, e.g. driven by make_1cycle(...).batch_step()) or any torch
+    `optimiser`: DeviceSGD, DeviceAdamW or DeviceMuon (hyper-parameters may change every step, e.g. driven by make_1cycle(...).batch_step()) or any torch
     optimiser whose step() is capturable with FIXED hyper-parameters (torch.optim.SGD(..., fused=True)).
     `valid_depth` (3D vs 2D loss per sample, train_3d.py:126-142) is fixed at capture time.
 
@@ -350,7 +635,7 @@ class PlannedTrainStep:
     What makes a replay valid: every tensor of the recorded iteration lives in a private allocator pool that stays reserved for
     this object (the replayed launches write the same addresses); everything the iteration computes is a launch of this library
     (the engine's fills and copies, the stage-loss sum, average_loss's backward, DeviceSGD) -- kernels of the tensor library
-    are not recorded; the backward pass is seeded with a persistent tensor of ones.  `optimiser` must be a DeviceSGD (its
+    are not recorded; the backward pass is seeded with a persistent tensor of ones.  `optimiser` must be a DeviceSGD, DeviceAdamW or DeviceMuon (its
     hyper-parameters live in device memory and may change every step); `valid_depth` must select one loss for the whole batch.
     Data parallel: the all-reduces of the gradient buckets are host actions -- the plan breaks at each, a replay issues them again
     between two segments (the same places the eager backward pass issues them).
@@ -358,8 +643,8 @@ class PlannedTrainStep:
 
     def __init__(self, model, optimiser, x, target, mask, valid_depth=None, warmup=2):
         import ctypes
-        if not isinstance(optimiser, DeviceSGD):
-            raise _lib.MposeError('PlannedTrainStep needs a DeviceSGD optimiser (torch optimisers launch kernels a plan cannot record)')
+        if not isinstance(optimiser, (DeviceSGD, DeviceAdamW, DeviceMuon)):
+            raise _lib.MposeError('PlannedTrainStep needs a DeviceSGD, DeviceAdamW or DeviceMuon optimiser (torch optimisers launch kernels a plan cannot record)')
         self.model, self.opt = model, optimiser
         self.x, self.target, self.mask = x.clone(), target.clone(), mask.clone()
         self.valid_depth = [1] * x.shape[0] if valid_depth is None else [int(v) for v in valid_depth]

@@ -1,0 +1,336 @@
+"""Orthogonalised updates on the GPU: train_helpers.orthogonalize, DeviceMuon and DeviceAdamW against plain float64 formulas.
+
+Tolerances (relative 2-norm against float64 of the SAME inputs).  Operands carry 22 bits (two fp16 values) and the l x l product is
+dropped: one product is off by at most u = 2^-22 of its operands' norms; sums are fp32.
+  * singular values of one size: signal and error are lifted alike.  Five steps are at most 17 products, each with two rounded operands
+    and one rounded result: 17 * 3 * u = 1.2e-5.
+  * any spectrum: an error u in S = X X^T is lifted by a^2 a step over the at most two steps that follow it in a group, and enters
+    Q = a I + b S + c S^2 times |b| + 2 |c| of a: u * a^4 * (|b| + 2 |c|) / a = 8.7e-5 of the small singular values' part, twice for the two
+    groups, plus X's own rounding (u a^5 |X0|_F = 1.2e-4 absolute, against |X|_F >= 0.6 where one singular value is 1).
+  * 16-bit outputs add their own half step: eps / 2 of the type."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from margipose_amd._lib import MposeError
+
+pytestmark = pytest.mark.gpu
+ABC = (3.4445, -4.7750, 2.0315)
+U = 2.0 ** -22
+TOL_FLAT = 17 * 3 * U
+TOL_ANY = 2 * U * ABC[0] ** 3 * (abs(ABC[1]) + 2 * abs(ABC[2])) + U * ABC[0] ** 5 / 0.6
+
+
+def _exact(g, steps=5, abc=ABC, eps=1e-7):
+    x = g.detach().double().cpu().reshape(g.shape[0], -1)
+    tall = x.shape[0] > x.shape[1]
+    x = x.T if tall else x
+    x = x / (x.norm() + eps)
+    a, b, c = abc
+    for _ in range(steps):
+        s = x @ x.T
+        x = a * x + (b * s + c * s @ s) @ x
+    return (x.T if tall else x).reshape(g.shape)
+
+
+def _rel(got, want):
+    got, want = got.detach().double().cpu(), want.double()
+    return float((got - want).norm() / want.norm().clamp_min(1e-300))
+
+
+def _flat(m, n, seed, lo=0.5):
+    """Singular values spread over [lo, 1]."""
+    g = torch.Generator().manual_seed(seed)
+    k = min(m, n)
+    u = torch.linalg.qr(torch.randn(m, k, generator=g, dtype=torch.float64))[0]
+    v = torch.linalg.qr(torch.randn(n, k, generator=g, dtype=torch.float64))[0]
+    return ((u * torch.linspace(lo, 1.0, k, dtype=torch.float64)) @ v.T).float()
+
+
+SHAPES = [(1, 1), (1, 5), (7, 1), (2, 3), (17, 128), (32, 27), (33, 31), (63, 65), (64, 64), (65, 63), (64, 1), (1, 200), (127, 130), (128, 1152),
+          (192, 192), (257, 96), (300, 40)]
+
+
+@pytest.mark.parametrize('shape', SHAPES)
+def test_one_matrix_of_flat_spectrum(shape):
+    from margipose_amd.train_helpers import orthogonalize
+    g = _flat(*shape, seed=shape[0] * 1000 + shape[1]).cuda()
+    keep = g.clone()
+    x = orthogonalize(g)
+    assert x.shape == g.shape and x.dtype == g.dtype and torch.equal(g, keep)
+    assert _rel(x, _exact(g)) <= TOL_FLAT
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('spectrum', ['decay', 'low_rank', 'one'])
+def test_uneven_spectra(spectrum, dtype):
+    from margipose_amd.train_helpers import orthogonalize
+    gen = torch.Generator().manual_seed(5)
+    for m, n in ((96, 200), (200, 96), (160, 160)):
+        k = min(m, n)
+        u = torch.linalg.qr(torch.randn(m, k, generator=gen, dtype=torch.float64))[0]
+        v = torch.linalg.qr(torch.randn(n, k, generator=gen, dtype=torch.float64))[0]
+        i = torch.arange(1, k + 1, dtype=torch.float64)
+        s = {'decay': 1 / i ** 2, 'low_rank': (i <= 4).double(), 'one': (i <= 1).double()}[spectrum]
+        g = (((u * s) @ v.T) * 3.0).to(dtype).cuda()
+        tol = TOL_ANY + (0.0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2)
+        x = orthogonalize(g)
+        assert x.dtype == dtype
+        assert _rel(x, _exact(g)) <= tol, (m, n)
+
+
+def test_a_set_of_shapes_equals_one_by_one():
+    """One call over many shapes runs the same tiles as a call each: equal bit for bit, in any order."""
+    from margipose_amd.train_helpers import orthogonalize
+    gen = torch.Generator().manual_seed(9)
+    mats = [torch.randn(*s, generator=gen).cuda() for s in SHAPES + [(130, 51), (17, 153), (640, 129)]] + [torch.randn(20, 4, 3, 3, generator=gen).cuda()]
+    alone = [orthogonalize(m) for m in mats]
+    for order in (list(range(len(mats))), list(range(len(mats)))[::-1]):
+        got = orthogonalize([mats[i] for i in order])
+        for i, x in zip(order, got):
+            assert torch.equal(x, alone[i])
+    again = orthogonalize(mats)
+    assert all(torch.equal(a, b) for a, b in zip(again, alone))
+    assert _rel(alone[-1], _exact(mats[-1])) <= TOL_ANY
+
+
+@pytest.mark.parametrize('count', [47, 48, 49, 130])
+def test_more_matrices_than_one_set_up_launch_takes(count):
+    from margipose_amd.train_helpers import orthogonalize
+    gen = torch.Generator().manual_seed(count)
+    mats = [torch.randn(3 + i % 5, 4 + i % 7, generator=gen).cuda() for i in range(count)]
+    got = orthogonalize(mats)
+    for i, (g, x) in enumerate(zip(mats, got)):
+        assert _rel(x, _exact(g)) <= TOL_ANY, i
+
+
+@pytest.mark.parametrize('steps,abc', [(1, ABC), (2, ABC), (3, ABC), (4, ABC), (6, ABC), (7, ABC), (12, (1.5, -0.5, 0.0)), (24, (1.5, -0.5, 0.0)), (3, (1.0, 0.0, 0.0)),
+                                       (2, (0.0, 1.0, 0.0)), (4, (-2.0, 1.5, -0.5))])
+def test_other_polynomials_and_step_counts(steps, abc):
+    """The flat-spectrum bound counts three products' roundings for each of the steps' four products, lifted by the largest slope that a
+    later step has for this polynomial where the slope exceeds the growth (|a| a step for the tiny singular values there are none of)."""
+    from margipose_amd.train_helpers import orthogonalize
+    g = _flat(40, 72, 3).cuda()
+    want = _exact(g, steps, abc)
+    got = orthogonalize(g, steps=steps, coefficients=abc)
+    assert _rel(got, want) <= (4 * steps + 3) * 3 * U
+
+
+@pytest.mark.parametrize('scale', [1e-38, 1e-30, 1e-12, 1e-7, 1.0, 1e20, 3e37])
+def test_any_magnitude(scale):
+    from margipose_amd.train_helpers import orthogonalize
+    g = (_flat(48, 80, 4) * 0.5).double().mul(scale).float().cuda()
+    got, want = orthogonalize(g), _exact(g)
+    assert torch.isfinite(got).all()
+    if scale >= 1e-12:            # (below: eps outweighs the norm by more than 2^45 or the floats are subnormal; results stay finite and small)
+        assert _rel(got, want) <= TOL_FLAT
+    else:
+        assert float(got.abs().max()) <= 2.0 * float(want.abs().max()) + 2.0 ** -60
+    g0 = orthogonalize(g, eps=0.0)
+    if scale > 1e-38:
+        assert _rel(g0, _exact(g, eps=0.0)) <= TOL_FLAT
+
+
+def test_zeros_nan_and_infinity_stay_in_their_matrix():
+    from margipose_amd.train_helpers import orthogonalize
+    mats = [_flat(70, 90, i).cuda() for i in range(4)]
+    clean = orthogonalize(mats)
+    mats[0].zero_()
+    mats[1][3, 70] = float('nan')
+    mats[2][69, 0] = float('inf')
+    got = orthogonalize(mats)
+    assert torch.equal(got[0], torch.zeros_like(got[0]))
+    assert torch.isnan(got[1]).all() and torch.isnan(got[2]).all()
+    assert torch.equal(got[3], clean[3])
+
+
+def test_views_streams_and_empty_inputs():
+    from margipose_amd.train_helpers import orthogonalize
+    gen = torch.Generator().manual_seed(21)
+    base = torch.randn(80, 121, generator=gen).cuda()
+    for v in (base[:, :97], base[3:50, 1:], base.t(), base[:, ::2], base.reshape(-1)[1:1 + 60 * 70].view(60, 70)):      # strided, transposed, off alignment
+        assert _rel(orthogonalize(v), _exact(v)) <= TOL_ANY
+    for v in (base.bfloat16().reshape(-1)[1:1 + 60 * 70].view(60, 70), base.half().reshape(-1)[3:3 + 61 * 71].view(61, 71)):
+        assert torch.equal(orthogonalize(v), orthogonalize(v.clone()))
+    assert orthogonalize([]) == []
+    e = orthogonalize([torch.zeros(0, 5, device='cuda'), base, torch.zeros(4, 0, device='cuda')])
+    assert e[0].shape == (0, 5) and e[2].shape == (4, 0) and torch.equal(e[1], orthogonalize(base))
+    want = orthogonalize(base)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = [orthogonalize(base) for _ in range(3)]
+    here = orthogonalize(base)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(g, want) for g in got + [here])
+
+
+def test_captured_graphs_share_no_scratch():
+    from margipose_amd.train_helpers import orthogonalize
+    gen = torch.Generator().manual_seed(22)
+    xs = [torch.randn(90, 140, generator=gen).cuda() for _ in range(2)]
+    graphs, outs = [], []
+    for x in xs:
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            orthogonalize(x)
+        torch.cuda.current_stream().wait_stream(side)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(orthogonalize(x))
+        graphs.append(g)
+    for it in range(3):
+        for x in xs:
+            x.copy_(torch.randn(90, 140, generator=gen))
+        want = [orthogonalize(x) for x in xs]
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in xs]
+        for s, g in zip(streams, graphs):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for o, w in zip(outs, want):
+            assert torch.equal(o, w), it
+
+
+# ---- the optimisers ----
+def _adamw_exact(p, g, m, v, t, lr, b1, b2, eps, wd):
+    m = b1 * m + (1 - b1) * g
+    v = b2 * v + (1 - b2) * g * g
+    return p - lr * (wd * p + (m / (1 - b1 ** t)) / (np.sqrt(v / (1 - b2 ** t)) + eps)), m, v
+
+
+@pytest.mark.parametrize('sizes', [[1], [5, 4096, 4097], [3] * 97, [192] * 5 + [1000003]])
+def test_adamw_follows_the_formula(sizes):
+    """Six roundings of fp32 a step and element, each half a step (2^-24) of p, of m or of the update (at most 5 lr)."""
+    from margipose_amd.train_helpers import DeviceAdamW, make_1cycle
+    gen = torch.Generator().manual_seed(sum(sizes))
+    ps = [torch.randn(n, generator=gen).cuda().requires_grad_(True) for n in sizes]
+    opt = DeviceAdamW(ps, lr=0.1, betas=(0.9, 0.99), weight_decay=0.05)
+    sched = make_1cycle(opt, 10, 0.1, 0.9)
+    ref = [[p.detach().double().cpu().numpy(), np.zeros(p.numel()), np.zeros(p.numel())] for p in ps]
+    for t in range(1, 5):
+        sched.batch_step()
+        gr = opt.param_groups[0]
+        for p, r in zip(ps, ref):
+            g = torch.randn(p.shape, generator=gen)
+            p.grad = g.cuda()
+            r[:] = _adamw_exact(r[0], g.double().numpy(), r[1], r[2], t, gr['lr'], gr['momentum'], gr['beta2'], gr['eps'], gr['weight_decay'])
+        version = ps[0]._version
+        opt.step()
+        assert ps[0]._version > version
+        for p, r in zip(ps, ref):
+            tol = t * 6 * 2.0 ** -24 * (np.abs(r[0]) + 5 * 0.1)
+            assert np.all(np.abs(p.detach().cpu().numpy() - r[0]) <= tol)
+
+
+def _muon_exact(p, g, buf, first, lr, mom, wd, nesterov, steps=5):
+    buf = g if first else mom * buf + g
+    u = g + mom * buf if nesterov else buf
+    return p * (1 - lr * wd) - lr * 0.2 * math.sqrt(max(p.shape[0], p.numel() // p.shape[0])) * _exact(u, steps), buf
+
+
+@pytest.mark.parametrize('nesterov', [True, False])
+def test_muon_follows_the_formula_under_a_schedule(nesterov):
+    """Per step the update is off by TOL_ANY of its norm and p by one rounding; the momentum by two.  Earlier steps' errors add up."""
+    from margipose_amd.train_helpers import DeviceMuon, make_1cycle
+    gen = torch.Generator().manual_seed(31)
+    shapes = [(64, 16, 3, 3), (48, 64), (17, 32, 1, 1), (5, 3), (128,), (1,), (16, 8, 3, 3)]
+    ps = [torch.randn(s, generator=gen).cuda().requires_grad_(True) for s in shapes]
+    extra = [torch.randn(30, 7, generator=gen).cuda().requires_grad_(True)]
+    opt = DeviceMuon(ps, lr=0.1, momentum=0.9, weight_decay=0.1, nesterov=nesterov, vectors=extra, vector_options={'betas': (0.9, 0.99)})
+    sched = make_1cycle(opt, 10, 0.1, 0.9)
+    assert [tuple(p.shape) for p in opt.param_groups[0]['params']] == [s for s in shapes if len(s) > 1]
+    mats, vecs = opt.param_groups[0]['params'], opt.param_groups[1]['params']
+    rm = [[p.detach().double().cpu(), None] for p in mats]
+    rv = [[p.detach().double().cpu().numpy(), np.zeros(p.shape), np.zeros(p.shape)] for p in vecs]
+    for t in range(1, 4):
+        sched.batch_step()
+        a, b = opt.param_groups
+        assert a['lr'] == b['lr'] and a['momentum'] == b['momentum']
+        for p, r in zip(mats, rm):
+            g = torch.randn(p.shape, generator=gen)
+            p.grad = g.cuda()
+            r[:] = _muon_exact(r[0], g.double(), r[1], t == 1, a['lr'], a['momentum'], a['weight_decay'], nesterov)
+        for p, r in zip(vecs, rv):
+            g = torch.randn(p.shape, generator=gen)
+            p.grad = g.cuda()
+            r[:] = _adamw_exact(r[0], g.double().numpy(), r[1], r[2], t, b['lr'], b['momentum'], b['beta2'], b['eps'], b['weight_decay'])
+        opt.step()
+        at = 0
+        for p, r in zip(mats, rm):
+            n = p.numel()
+            update = 0.1 * 0.2 * math.sqrt(max(p.shape[0], n // p.shape[0])) * math.sqrt(min(p.shape[0], n // p.shape[0]))
+            tol = t * (2.0 ** -23 * float(r[0].norm()) + TOL_ANY * update * 1.2)
+            assert float((p.detach().double().cpu() - r[0]).norm()) <= tol, tuple(p.shape)
+            buf = opt.momentum_arena[at:at + n].view(p.shape)
+            assert _rel(buf, r[1]) <= t * 2.0 ** -23
+            at += (n + 3) // 4 * 4
+        for p, r in zip(vecs, rv):
+            assert np.all(np.abs(p.detach().cpu().numpy() - r[0]) <= t * 6 * 2.0 ** -24 * (np.abs(r[0]) + 0.5))
+
+
+def test_state_dict_resumes_bit_for_bit():
+    from margipose_amd.train_helpers import DeviceMuon
+    gen = torch.Generator().manual_seed(41)
+    shapes = [(20, 30), (7, 3, 3, 3), (11,)]
+    start = [torch.randn(s, generator=gen) for s in shapes]
+    grads = [[torch.randn(s, generator=gen) for s in shapes] for _ in range(4)]
+
+    def steps(ps, opt, some):
+        for gs in some:
+            for p, g in zip(ps, gs):
+                p.grad = g.cuda()
+            opt.step()
+
+    pa = [t.cuda().requires_grad_(True) for t in start]
+    oa = DeviceMuon(pa, lr=0.05)
+    steps(pa, oa, grads)
+    pb = [t.cuda().requires_grad_(True) for t in start]
+    ob = DeviceMuon(pb, lr=0.05)
+    steps(pb, ob, grads[:2])
+    pc = [p.detach().clone().requires_grad_(True) for p in pb]
+    oc = DeviceMuon(pc, lr=1.0, momentum=0.1)
+    oc.load_state_dict(ob.state_dict())
+    steps(pc, oc, grads[2:])
+    for a, c in zip(pa, pc):
+        assert torch.equal(a, c)
+
+
+def test_refusals_on_the_device():
+    from margipose_amd.train_helpers import DeviceAdamW, DeviceMuon, orthogonalize
+    m = torch.randn(4, 5, device='cuda')
+    with pytest.raises(MposeError, match='two dimensions'):
+        orthogonalize(m[0])
+    with pytest.raises(MposeError, match='one device and one of'):
+        orthogonalize([m, m.half()])
+    with pytest.raises(MposeError, match='one device and one of'):
+        orthogonalize(m.double())
+    with pytest.raises(MposeError, match='not differentiable'):
+        orthogonalize(m.clone().requires_grad_(True))
+    for bad in (dict(steps=0), dict(steps=25), dict(eps=-1.0), dict(eps=float('nan')), dict(coefficients=(9.0, 1.0, 1.0)), dict(coefficients=(float('inf'), 0, 0))):
+        with pytest.raises(MposeError, match='refused'):
+            orthogonalize(m, **bad)
+    with pytest.raises(MposeError, match='three numbers'):
+        orthogonalize(m, coefficients=(1.0, 2.0))
+    p = m.clone().requires_grad_(True)
+    with pytest.raises(MposeError, match='once'):
+        DeviceMuon([p, p])
+    with pytest.raises(MposeError, match='at least one'):
+        DeviceMuon([torch.zeros(3, device='cuda')])
+    with pytest.raises(MposeError, match='float32'):
+        DeviceAdamW([torch.zeros(3, device='cuda').half()])
+    opt = DeviceMuon([p])
+    with pytest.raises(RuntimeError, match='no gradient'):
+        opt.step()
+    p.grad = torch.randn(5, 4, device='cuda').t()
+    with pytest.raises(RuntimeError, match='contiguous gradients'):
+        opt.step()
+    p.grad = torch.randn(4, 5, device='cuda')
+    p.data = torch.randn(5, 4, device='cuda').t()
+    with pytest.raises(MposeError, match='contiguous parameters'):
+        opt.step()
