@@ -6,9 +6,10 @@
 // they commute, they are symmetric, and the next S is Q S Q without touching X.  So the long axis is visited twice per GROUP of steps,
 //     S = X X^T;   per step: Q = q(S), W = Q S, S <- W Q, P <- Q P;   X <- P X,
 // and every m x m product computes only the tiles on and above the diagonal (the others are their transposes).
-// In a group the rounding of S is lifted by a^2 a step where s is small: groups are as long as a^2 to the power (length - 1) stays
-// below 150 (3 + 2 steps for the customary a = 3.4445).  Relative error against float64 of one 256 x 256 matrix with
-// slowly decaying singular values, in a model of the arithmetic: one group of five 1e-4, groups of 3 + 2 and X on every step 4e-6.
+// In a group the rounding of S is lifted by a^2 a step where s is small, so a group is as long as a^2 to the power (length - 1) stays below
+// a limit: 12 for mpose_orthogonalize (groups of 2, 2, 1 for the customary a = 3.4445), 150 for mpose_muon_step (3, 2), whose result is
+// a small part of a weight.  Relative error against float64, 128 x 1152, decaying singular values: one group of five 1e-4, (3, 2)
+// 3.4e-6, (2, 2, 1) as X on every step in fp32, 1.4e-6.  Visits of the long axis: 2 against 3.
 //
 // Arithmetic: like the convolutions (three fp16 products of two-way split operands, x * 2^k = h + l: 22 bits), but the scale
 // exponents come from a bound, not from a measurement: |x_ij| <= |X|_2, and a scalar recursion bounds |X|_2, |S|_2, |Q|_2 from the
@@ -524,54 +525,60 @@ __global__ __launch_bounds__(256, 2) void orth_gemm_k(GemmArgs a) {
       d1 = j.t[a.parity ^ 1]; rp1 = j.cp; lim1 = j.rows; k1 = j.rk;
       d2 = j.n[a.parity ^ 1]; rp2 = j.rp; lim2 = j.cols; k2 = j.ck;
     }
-    const bool second = KIND == K_X || i0 != j0;      // (a diagonal tile holds both halves itself)
     __syncthreads();                                   // the ring becomes the transposing buffer
     float* tr = reinterpret_cast<float*>(smem) + wave * 32 * 33;
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
       for (int c = 0; c < R; ++c) {
-        const int col = jb + c * 32 + li;
+        const int rb = ib + r * 32, cb = jb + c * 32;
+        // A symmetric product is written once and mirrored: blocks under the diagonal are skipped, a block on it takes its own upper half
+        // twice.  (Left as computed, the halves differ by their roundings, and a product with such a matrix is not S^2 but S S^T: from the
+        // third step of a group on the error grew tenfold.)
+        if (KIND != K_X && rb > cb) continue;
+        const bool diag = KIND != K_X && rb == cb;
+        float x[16];
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const int k = ib + r * 32 + 8 * g + 4 * lh;
-          float x[4];
-#pragma unroll
-          for (int v = 0; v < 4; ++v) x[v] = (acc[r][c][4 * g + v] + acx[r][c][4 * g + v]) * da * db;
-          if constexpr (KIND == K_Q) {
-            if (k < j.mk) {
-              const unsigned char* sp = j.s + (((long)(k >> 3) * 2 * j.mp + col) * 16 + (k & 4) * 2);
-              const f16x4 sh = *reinterpret_cast<const f16x4*>(sp), sl = *reinterpret_cast<const f16x4*>(sp + (long)j.mp * 16);
-#pragma unroll
-              for (int v = 0; v < 4; ++v) {
-                const float s = ((float)sh[v] + (float)sl[v]) * da;
-                x[v] = fmaf(a.k.c, x[v], a.k.b * s) + (k + v == col ? a.k.a : 0.f);
-              }
-            }
-          }
-#pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            x[v] *= so;
-            tr[(8 * g + 4 * lh + v) * 33 + li] = x[v];
-            if (k + v >= lim1) x[v] = 0.f;
-          }
-          if (k < k1) put4(d1, rp1, col, k, x);
-        }
-        if (second) {
-          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // (one wave: its LDS accesses execute in order)
-          const int row = ib + r * 32 + li;
+        for (int v = 0; v < 16; ++v) x[v] = (acc[r][c][v] + acx[r][c][v]) * da * db;
+        if constexpr (KIND == K_Q) {
+          const int col = cb + li;
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
-            const int k = jb + c * 32 + 8 * g + 4 * lh;
-            float x[4];
+            const int k = rb + 8 * g + 4 * lh;
+            if (k >= j.mk) continue;
+            const unsigned char* sp = j.s + (((long)(k >> 3) * 2 * j.mp + col) * 16 + (k & 4) * 2);
+            const f16x4 sh = *reinterpret_cast<const f16x4*>(sp), sl = *reinterpret_cast<const f16x4*>(sp + (long)j.mp * 16);
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
-              x[v] = tr[li * 33 + 8 * g + 4 * lh + v];
-              if (k + v >= lim2) x[v] = 0.f;
+              const float s = ((float)sh[v] + (float)sl[v]) * da;
+              x[4 * g + v] = fmaf(a.k.c, x[4 * g + v], a.k.b * s) + (k + v == col ? a.k.a : 0.f);
             }
-            if (k < k2) put4(d2, rp2, row, k, x);
           }
-          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          x[v] *= so;
+          tr[(8 * (v >> 2) + 4 * lh + (v & 3)) * 33 + li] = x[v];
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // (one wave: its LDS accesses execute in order)
+        float y[16];                                            // the block's transpose: row rb + li, columns cb + 8 g + 4 lh + v
+#pragma unroll
+        for (int v = 0; v < 16; ++v) y[v] = tr[li * 33 + 8 * (v >> 2) + 4 * lh + (v & 3)];
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int o = 8 * g + 4 * lh;
+          float u[4];
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            u[v] = diag && o + v > li ? y[4 * g + v] : x[4 * g + v];
+            if (rb + o + v >= lim1) u[v] = 0.f;
+          }
+          if (rb + o < k1) put4(d1, rp1, cb + li, rb + o, u);
+          if (diag) continue;
+#pragma unroll
+          for (int v = 0; v < 4; ++v) u[v] = cb + o + v < lim2 ? y[4 * g + v] : 0.f;
+          if (cb + o < k2) put4(d2, rp2, rb + li, cb + o, u);
         }
       }
   }
@@ -580,10 +587,10 @@ __global__ __launch_bounds__(256, 2) void orth_gemm_k(GemmArgs a) {
 // ---- host ----
 struct Groups { int n, first[kMaxSteps], size[kMaxSteps], mask; };
 
-Groups make_groups(int steps, float a) {
+Groups make_groups(int steps, float a, double limit) {
   const double a2 = (double)a * a;
   int longest = 1;
-  for (double lift = a2; lift <= 150.0 && longest < steps; lift *= a2 > 1.0 ? a2 : 1.0) ++longest;
+  for (double lift = a2; lift <= limit && longest < steps; lift *= a2 > 1.0 ? a2 : 1.0) ++longest;
   Groups g{};
   g.n = (steps + longest - 1) / longest;
   int at = 0;
@@ -603,7 +610,7 @@ struct OrthPlan {
   Groups g;
 };
 
-int make_plan(const mpose_orth_job* jobs, int n_jobs, const mpose_orth_options* o, OrthPlan& p) {
+int make_plan(const mpose_orth_job* jobs, int n_jobs, const mpose_orth_options* o, bool muon, OrthPlan& p) {
   if (n_jobs < 0 || n_jobs > 65535 || !o || (n_jobs > 0 && !jobs)) return MPOSE_EINVAL;
   if (o->steps < 1 || o->steps > kMaxSteps || o->dtype < 0 || o->dtype > 2 || !(o->eps >= 0.f) || !isfinite(o->eps)) return MPOSE_EINVAL;
   if (!isfinite(o->a) || !isfinite(o->b) || !isfinite(o->c)) return MPOSE_EINVAL;
@@ -615,7 +622,7 @@ int make_plan(const mpose_orth_job* jobs, int n_jobs, const mpose_orth_options* 
     if (!(bx <= kGrowth)) return MPOSE_EINVAL;
   }
   p = OrthPlan{};
-  p.g = make_groups(o->steps, o->a);
+  p.g = make_groups(o->steps, o->a, muon ? 150.0 : 12.0);
   p.tile = 64;
   int64_t body = 0;
   for (int i = 0; i < n_jobs; ++i) {
@@ -646,7 +653,7 @@ void gemm(const GemmArgs& a, int ny, hipStream_t s) {
 int run(const mpose_orth_job* jobs, int n_jobs, const mpose_orth_options* o, bool muon, const Hyper& h, const float* hyper_dev, void* ws, int64_t ws_bytes,
         hipStream_t s) {
   OrthPlan p;
-  const int rc = make_plan(jobs, n_jobs, o, p);
+  const int rc = make_plan(jobs, n_jobs, o, muon, p);
   if (rc != 0) return rc;
   if (n_jobs == 0) return 0;
   if (!ws || ((uintptr_t)ws & 255) || ws_bytes < p.total_b) return MPOSE_EINVAL;
@@ -729,9 +736,11 @@ int run(const mpose_orth_job* jobs, int n_jobs, const mpose_orth_options* o, boo
 using namespace mpose;
 
 extern "C" int64_t mpose_orth_ws_bytes(const mpose_orth_job* jobs, int n_jobs, const mpose_orth_options* options) {
-  OrthPlan p;
-  const int rc = make_plan(jobs, n_jobs, options, p);
-  return rc != 0 ? (int64_t)rc : p.total_b;
+  OrthPlan p, q;
+  int rc = make_plan(jobs, n_jobs, options, false, p);
+  if (rc == 0) rc = make_plan(jobs, n_jobs, options, true, q);
+  if (rc != 0) return rc;
+  return p.total_b > q.total_b ? p.total_b : q.total_b;
 }
 
 extern "C" int mpose_orthogonalize(const mpose_orth_job* jobs, int n_jobs, const mpose_orth_options* options, void* ws, int64_t ws_bytes, void* stream) {
