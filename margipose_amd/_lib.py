@@ -24,6 +24,9 @@ MAX_TAPS = 12
 MAX_CLASSES = 8
 
 
+IO_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}       # the C ABI's io_dtype / w_dtype / dtype
+
+
 class MposeError(RuntimeError):
     pass
 
@@ -47,6 +50,11 @@ def lib():
         _LIB.mpose_orthogonalize.argtypes = [c_void_p, c_int, c_void_p, c_void_p, c_int64, c_void_p]
         _LIB.mpose_muon_step.argtypes = [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]
         _LIB.mpose_adamw_step.argtypes = [c_void_p, c_int, c_void_p, c_void_p, c_void_p]
+        _LIB.mpose_layer_norm_fwd.argtypes = [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_float, c_int, c_int, c_void_p]
+        _LIB.mpose_layer_norm_bwd_ws_bytes.restype = c_int64
+        _LIB.mpose_layer_norm_bwd_ws_bytes.argtypes = [c_int64, c_int]
+        _LIB.mpose_layer_norm_bwd.argtypes = [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int,
+                                              c_int, c_int, c_void_p, c_int64, c_void_p]
         _LIB.mpose_set8.argtypes = [c_void_p, c_void_p, c_void_p]
     return _LIB
 

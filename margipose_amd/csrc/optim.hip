@@ -129,6 +129,7 @@ extern "C" int mpose_set8(float* dst, const float* src8, void* stream) {
 
 extern "C" int mpose_adamw_step(const mpose_adamw_job* jobs, int n_jobs, const float* hyper, const float* hyper_dev, void* stream) {
   if (n_jobs < 0 || (n_jobs > 0 && !jobs) || (!hyper && !hyper_dev)) return MPOSE_EINVAL;
+  if (n_jobs == 0) return 0;
   for (int i = 0; i < n_jobs; ++i) {
     const mpose_adamw_job& j = jobs[i];
     if (j.n < 0 || (j.n > 0 && (!j.p || !j.g || !j.m || !j.v))) return MPOSE_EINVAL;
@@ -147,7 +148,7 @@ extern "C" int mpose_adamw_step(const mpose_adamw_job* jobs, int n_jobs, const f
       }
       ++at;
     }
-    if (a.n == 0) break;
+    if (a.n == 0) return 0;              // (only arrays of no elements are left)
     int64_t bx = (longest + kAdamChunk - 1) / kAdamChunk;
     if (bx > 1024) bx = 1024;
     launch(adamw_step_k, dim3((unsigned)bx, (unsigned)a.n), dim3(256), 0, (hipStream_t)stream, a);

@@ -268,7 +268,6 @@ class DeviceSGD:
             g.update(s)
 
 
-IO_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 MUON_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 _ORTH_JOB_DT = [('src', 'u8'), ('buf', 'u8'), ('dst', 'u8'), ('rows', 'i4'), ('cols', 'i4'), ('scale', 'f4'), ('reserved', 'i4')]
 _ADAMW_JOB_DT = [('p', 'u8'), ('g', 'u8'), ('m', 'u8'), ('v', 'u8'), ('n', 'i8')]
@@ -293,7 +292,7 @@ def _orth_options(steps, coefficients, eps, dtype, nesterov=False):
         a, b, c = (float(v) for v in coefficients)
     except (TypeError, ValueError):
         raise _lib.MposeError('Newton-Schulz coefficients are three numbers (a, b, c), got %r' % (coefficients,))
-    return _lib.OrthOptions(int(steps), IO_DTYPES[dtype], int(bool(nesterov)), 0, a, b, c, float(eps))
+    return _lib.OrthOptions(int(steps), _lib.IO_DTYPES[dtype], int(bool(nesterov)), 0, a, b, c, float(eps))
 
 
 def _orth_workspace_bytes(jobs, options):
@@ -322,7 +321,7 @@ def orthogonalize(matrices, steps=5, coefficients=MUON_COEFFICIENTS, eps=1e-7):
             raise _lib.MposeError('orthogonalize needs tensors of at least two dimensions')
         if not t.is_cuda:
             raise _lib.MposeError('orthogonalize: matrices must live on a ROCm device (got %s): margipose_amd has no CPU path' % t.device)
-        if t.dtype != first.dtype or t.device != first.device or t.dtype not in IO_DTYPES:
+        if t.dtype != first.dtype or t.device != first.device or t.dtype not in _lib.IO_DTYPES:
             raise _lib.MposeError('orthogonalize: matrices must share one device and one of float32, bfloat16, float16')
         if t.requires_grad and torch.is_grad_enabled():
             raise _lib.MposeError('orthogonalize is not differentiable: pass detached tensors or call it under torch.no_grad()')
