@@ -58,10 +58,10 @@ struct OrthLayout {                     // byte offsets inside a job's part of t
 
 __host__ __device__ inline int pad_to(int v, int q) { return (v + q - 1) / q * q; }
 
-__host__ __device__ inline OrthLayout orth_layout(int rows, int cols, int tile, int n_groups) {
+__host__ __device__ inline OrthLayout orth_layout(int rows, int cols, int pad, int n_groups) {
   OrthLayout l;
   const int m = rows < cols ? rows : cols;
-  l.rp = pad_to(rows, tile); l.cp = pad_to(cols, tile); l.mp = pad_to(m, tile);
+  l.rp = pad_to(rows, pad); l.cp = pad_to(cols, pad); l.mp = pad_to(m, pad);
   l.rk = pad_to(rows, 32); l.ck = pad_to(cols, 32); l.mk = pad_to(m, 32);
   l.n_part = (int)(((int64_t)rows * cols + kChunk - 1) / kChunk);
   const int64_t nb = (int64_t)l.ck * l.rp * 4, tb = (int64_t)l.rk * l.cp * 4, mb = (int64_t)l.mk * l.mp * 4;
@@ -92,13 +92,27 @@ struct SetupArgs {
   SetupJob j[kSetupJobs];
   OrthJob* jobs;
   int2 *ew, *split, *sym, *fin;
-  int first, n, tile, n_groups, elem;
+  int first, n, pad, tile_sym, tile_fin, n_groups, elem;
 };
+
+// Order of the tiles of one product: 8 x 8 blocks of tiles one after another, so that the tiles that an XCD holds at a time share their rows
+// of both operands in its 4 MB of L2 (row after row, a 4096 x 4096 product fetched 1.6 GB through the fabric).
+constexpr int kBlock = 8;
+__device__ inline int block_place(int r, int c, int tr, int tc) {
+  const int R = r / kBlock, C = c / kBlock, dr = min(kBlock, tr - R * kBlock), dc = min(kBlock, tc - C * kBlock);
+  return R * kBlock * tc + C * kBlock * dr + (r - R * kBlock) * dc + (c - C * kBlock);
+}
+__device__ inline int upper_place(int r, int c, int t) {          // ... of the tiles on and above the diagonal
+  const int R = r / kBlock, C = c / kBlock, r0 = R * kBlock, d = min(kBlock, t - r0), lr = r - r0, lc = c - C * kBlock;
+  const int before = r0 * t - r0 * (r0 - 1) / 2;
+  if (C == R) return before + lr * d - lr * (lr - 1) / 2 + (lc - lr);
+  return before + d * (d + 1) / 2 + (C - R - 1) * d * kBlock + lr * min(kBlock, t - C * kBlock) + lc;
+}
 
 __global__ __launch_bounds__(256) void orth_setup_k(SetupArgs a) {
   const SetupJob& j = a.j[blockIdx.x];
   const int id = a.first + blockIdx.x;
-  const OrthLayout l = orth_layout(j.rows, j.cols, a.tile, a.n_groups);
+  const OrthLayout l = orth_layout(j.rows, j.cols, a.pad, a.n_groups);
   if (threadIdx.x == 0) {
     OrthJob* o = a.jobs + id;
     o->src = j.src; o->buf = j.buf; o->dst = j.dst; o->scale = j.scale;
@@ -116,13 +130,16 @@ __global__ __launch_bounds__(256) void orth_setup_k(SetupArgs a) {
   for (int i = threadIdx.x; i < l.n_part; i += 256) a.ew[j.ew0 + i] = make_int2(id, i);
   const int sr = (j.rows + 63) / 64, sc = (j.cols + 63) / 64;
   for (int i = threadIdx.x; i < sr * sc; i += 256) a.split[j.split0 + i] = make_int2(id, (i / sc) | ((i % sc) << 16));
-  const int tm = l.mp / a.tile;
-  for (int i = threadIdx.x; i < tm * tm; i += 256) {             // row-major over the upper triangle
+  const int m = j.rows < j.cols ? j.rows : j.cols, tm = (m + a.tile_sym - 1) / a.tile_sym;
+  for (int i = threadIdx.x; i < tm * tm; i += 256) {
     const int r = i / tm, c = i % tm;
-    if (c >= r) a.sym[j.sym0 + r * tm - r * (r - 1) / 2 + (c - r)] = make_int2(id, r | (c << 16));
+    if (c >= r) a.sym[j.sym0 + upper_place(r, c, tm)] = make_int2(id, r | (c << 16));
   }
-  const int tr = l.rp / a.tile, tc = l.cp / a.tile;
-  for (int i = threadIdx.x; i < tr * tc; i += 256) a.fin[j.fin0 + i] = make_int2(id, (i / tc) | ((i % tc) << 16));
+  const int tr = (j.rows + a.tile_fin - 1) / a.tile_fin, tc = (j.cols + a.tile_fin - 1) / a.tile_fin;
+  for (int i = threadIdx.x; i < tr * tc; i += 256) {
+    const int r = i / tc, c = i % tc;
+    a.fin[j.fin0 + block_place(r, c, tr, tc)] = make_int2(id, r | (c << 16));
+  }
 }
 
 // ---- element access ----
@@ -259,13 +276,24 @@ __device__ __forceinline__ int exp_of(float bound) {
   return k > 60 ? 60 : k;
 }
 
-// ---- pass 2: one wave per matrix: |G|_F, the input scale, every step's scale exponents ----
-__global__ __launch_bounds__(64) void orth_scalars_k(OrthJob* jobs, Poly k, double eps, int steps, int group_first_mask) {
+// ---- pass 2: one workgroup per matrix: |G|_F, the input scale, every step's scale exponents ----
+__global__ __launch_bounds__(256) void orth_scalars_k(OrthJob* jobs, Poly k, double eps, int steps, int group_first_mask) {
   OrthJob& j = jobs[blockIdx.x];
+  __shared__ double sh[4];
   double s = 0.0;
-  for (int i = threadIdx.x; i < j.n_part; i += 64) s += j.part[i];
+  const int n = j.n_part;
+  const double* const part = j.part;
+  int at = threadIdx.x;
+  for (; at + 768 < n; at += 1024) {              // four partial sums in flight
+    const double v0 = part[at], v1 = part[at + 256], v2 = part[at + 512], v3 = part[at + 768];
+    s += (v0 + v1) + (v2 + v3);
+  }
+  for (; at < n; at += 256) s += part[at];
   s = wave_sum(s);
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = s;
+  __syncthreads();
   if (threadIdx.x != 0) return;
+  s = sh[0] + sh[1] + sh[2] + sh[3];
   const double norm = sqrt(s), den = norm + eps;
   float bx = norm > 0.0 ? (float)(norm / den) : 0.f, bp = 1.f;
   StepExp e{0, 0, 0, 0, 0};
@@ -354,9 +382,11 @@ enum { K_GRAM = 0, K_Q = 1, K_MUL = 2, K_NEXT = 3, K_X = 4, K_OUT = 5 };
 struct GemmArgs {
   const OrthJob* jobs;
   const int2* list;
-  int n_tiles;
+  int n_tiles, n_main;                // tiles of the list; of the n_tiles (x 2) tiles of the launch, those with a workgroup each
+  int split;                          // workgroups for each of the others, which leave their shares of the sum in `part`
+  float* part;
   int step, step0, i, parity;         // step; the group's first step; step - step0; the group's X set
-  int y0;                             // K_MUL: first of {W = Q S, P = Q P} that grid.y counts from
+  int y0;                             // K_MUL: which of {W = Q S, P = Q P} comes first
   Poly k;
   Hyper h;
   const float* hyper_dev;
@@ -380,18 +410,36 @@ __device__ __forceinline__ void put4(unsigned char* base, int rp, int row, int k
 
 // C = A B^T over H8 operands, one 64 R x 64 R tile per workgroup: 2 x 2 waves, R x R accumulator blocks of 32 x 32 per wave.
 // Per k = 16: 4 R fragment reads for 3 R^2 MFMAs.  Ring of NBUF slots of k = 32, filled by LDS DMA.
-template <int R, int NBUF, int KIND, int DT>
-__global__ __launch_bounds__(256, 2) void orth_gemm_k(GemmArgs a) {
+// JOIN: no product, the tile's sum is that of its `split` partial sums, added in their order.
+template <int R, int NBUF, int KIND, int DT, bool JOIN>
+__global__ __launch_bounds__(256, NBUF * R > 4 ? 1 : 2) void orth_gemm_k(GemmArgs a) {
   constexpr int T = 64 * R;
   constexpr int kOp = 8 * T * 16, kSlot = 2 * kOp;        // bytes of one operand / both in a slot: [octet 4][plane 2][T][16 B]
   constexpr int LW = 4 * R;                               // DMA instructions per wave and slot
-  __shared__ __attribute__((aligned(16))) unsigned char smem[NBUF * kSlot];
-  static_assert(4 * 32 * 33 * 4 <= NBUF * kSlot, "the transposing epilogue fits the ring");
-  // workgroup b runs on XCD b % 8 (observed placement, speed only): an XCD takes a contiguous run of the tile list
-  const int per = (a.n_tiles + 7) >> 3;
-  const int idx = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
-  if (idx >= a.n_tiles) return;
-  const int2 it = a.list[idx];
+  constexpr int kLds = JOIN ? 4 * 32 * 33 * 4 : NBUF * kSlot;
+  __shared__ __attribute__((aligned(16))) unsigned char smem[kLds];
+  static_assert(4 * 32 * 33 * 4 <= kLds, "the transposing epilogue fits the ring");
+  constexpr int RA = JOIN ? 1 : R;                        // accumulator blocks each way: a join takes one of its tile's R x R sets of four
+  int idx, share = 0, set = 0;
+  bool partial = false;
+  if constexpr (JOIN) {
+    idx = a.n_main + (int)blockIdx.x / (R * R);
+    set = (int)blockIdx.x % (R * R);
+  } else {
+    // workgroup b runs on XCD b % 8 (observed placement, speed only): an XCD takes a contiguous run of the tile list
+    const int per = (a.n_main + 7) >> 3, b = (int)blockIdx.x;
+    if (b < per * 8) {
+      idx = (b & 7) * per + (b >> 3);
+      if (idx >= a.n_main) return;
+    } else {
+      const int q = (b - per * 8) / a.split;
+      share = (b - per * 8) - q * a.split;
+      idx = a.n_main + q;
+      partial = true;
+    }
+  }
+  const int second_half = idx >= a.n_tiles ? 1 : 0;
+  const int2 it = a.list[idx - second_half * a.n_tiles];
   const OrthJob& j = a.jobs[it.x];
   const int i0 = (it.y & 0xffff) * T, j0 = (int)((unsigned)it.y >> 16) * T;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -409,7 +457,7 @@ __global__ __launch_bounds__(256, 2) void orth_gemm_k(GemmArgs a) {
   } else if constexpr (KIND == K_Q) {
     A = B = j.s; ea = eb = e.s; eo = e.q; out = j.q[a.i & 1];
   } else if constexpr (KIND == K_MUL) {
-    const bool p = a.y0 + (int)blockIdx.y != 0;
+    const bool p = a.y0 + second_half != 0;
     unsigned char* const prev = a.i == 1 ? j.q[0] : j.p[(a.i + 1) & 1];
     unsigned char* const next = j.p[a.i & 1];
     A = j.q[a.i & 1]; ea = e.q;
@@ -428,16 +476,28 @@ __global__ __launch_bounds__(256, 2) void orth_gemm_k(GemmArgs a) {
     if (KIND == K_X) eo = j.e[a.step + 1].x;
   }
 
-  f32x16 acc[R][R], acx[R][R];          // h x h, and the two cross products (2^-11 of it: their roundings do not matter)
+  f32x16 acc[RA][RA], acx[RA][RA];      // h x h, and the two cross products (2^-11 of it: their roundings do not matter)
 #pragma unroll
-  for (int r = 0; r < R; ++r)
+  for (int r = 0; r < RA; ++r)
 #pragma unroll
-    for (int c = 0; c < R; ++c)
+    for (int c = 0; c < RA; ++c)
 #pragma unroll
       for (int v = 0; v < 16; ++v) { acc[r][c][v] = 0.f; acx[r][c][v] = 0.f; }
 
-  const int n_slots = kk >> 5;
-  {
+  constexpr int NQ = R * R * 4;                            // float4s of a thread's share of the tile
+  if constexpr (JOIN) {
+    const float4* p = reinterpret_cast<const float4*>(a.part) + ((long)(idx - a.n_main) * a.split * NQ + set * 4) * 256 + tid;
+#pragma unroll 4
+    for (int q = 0; q < a.split; ++q) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const float4 v = p[((long)q * NQ + g) * 256];
+        acc[0][0][4 * g] += v.x; acc[0][0][4 * g + 1] += v.y; acc[0][0][4 * g + 2] += v.z; acc[0][0][4 * g + 3] += v.w;
+      }
+    }
+  } else {
+    // the slots of this workgroup: all, or its share of a tile that is split
+    const int all = kk >> 5, s_lo = partial ? (int)((long)all * share / a.split) : 0, n_slots = (partial ? (int)((long)all * (share + 1) / a.split) : all) - s_lo;
     // waves 0, 1 fetch A, waves 2, 3 fetch B; each half of the operand's eight (octet, plane) slabs
     const bool isb = wave >= 2;
     const int rp = isb ? brp : arp, row0 = isb ? j0 : i0;
@@ -450,68 +510,109 @@ __global__ __launch_bounds__(256, 2) void orth_gemm_k(GemmArgs a) {
 #pragma unroll
       for (int u = 0; u < LW; ++u) {
         const int sl = u / R, rg = u % R;
-        const unsigned soff = ((unsigned)s * 8u + (unsigned)((wave & 1) * 4 + sl)) * slab + (unsigned)(row0 + rg * 64) * 16u;
+        const unsigned soff = ((unsigned)(s_lo + s) * 8u + (unsigned)((wave & 1) * 4 + sl)) * slab + (unsigned)(row0 + rg * 64) * 16u;
         __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void_p)(l + u * 1024), 16, (int)voff, (int)soff, 0, 0);
       }
+    };
+    // The loop always reads the fragments of the next k = 16 before it multiplies the current ones: two register sets, F0 for the
+    // first half of a slot, F1 for the second.  One barrier per slot, passed while F1 still has to be multiplied.
+    struct Frags { f16x8 ah[R], al[R], bh[R], bl[R]; } f0, f1;
+    const unsigned char* const pa = smem + (wm * 32 * R + li) * 16 + lh * 2 * T * 16;
+    const unsigned char* const pb = smem + kOp + (wn * 32 * R + li) * 16 + lh * 2 * T * 16;
+    auto read = [&](Frags& f, int s, int k16) {
+      const int o = (s % NBUF) * kSlot + k16 * 4 * T * 16;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        f.ah[r] = *reinterpret_cast<const f16x8*>(pa + o + r * 512);
+        f.bh[r] = *reinterpret_cast<const f16x8*>(pb + o + r * 512);
+        f.bl[r] = *reinterpret_cast<const f16x8*>(pb + o + T * 16 + r * 512);
+        f.al[r] = *reinterpret_cast<const f16x8*>(pa + o + T * 16 + r * 512);
+      }
+    };
+    auto multiply = [&](const Frags& f) {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int c = 0; c < R; ++c) {
+          acx[r][c] = mfma(f.ah[r], f.bl[c], acx[r][c]);
+          acc[r][c] = mfma(f.ah[r], f.bh[c], acc[r][c]);
+          acx[r][c] = mfma(f.al[r], f.bh[c], acx[r][c]);
+        }
+    };
+    auto enter = [&](int s) {                      // slot s becomes readable, slot s - 1 writable
+      if (s + NBUF - 2 < n_slots) wait_vm<LW * (NBUF - 2)>();
+      else wait_vm<0>();
+      __builtin_amdgcn_s_waitcnt(0xC07F);          // lgkmcnt(0): this wave's reads of slot s - 1 are in registers
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if (s + NBUF - 1 < n_slots) fetch(s + NBUF - 1);
     };
 #pragma unroll
     for (int s = 0; s < NBUF - 1; ++s)
       if (s < n_slots) fetch(s);
+    if (n_slots > 0) {
+      enter(0);
+      read(f0, 0, 0);
+    }
     for (int s = 0; s < n_slots; ++s) {
-      if (s + NBUF - 2 < n_slots) wait_vm<LW * (NBUF - 2)>();
-      else wait_vm<0>();
-      __builtin_amdgcn_s_waitcnt(0xC07F);          // lgkmcnt(0): this wave's reads of slot s - 1 are in registers
-      __builtin_amdgcn_s_barrier();                // slot s is whole, slot s - 1 is free
-      asm volatile("" ::: "memory");
-      if (s + NBUF - 1 < n_slots) fetch(s + NBUF - 1);
-      const unsigned char* pa = smem + (s % NBUF) * kSlot + (wm * 32 * R + li) * 16;
-      const unsigned char* pb = smem + (s % NBUF) * kSlot + kOp + (wn * 32 * R + li) * 16;
-#pragma unroll
-      for (int k16 = 0; k16 < 2; ++k16) {
-        f16x8 ah[R], al[R], bh[R], bl[R];
-        const int o = (k16 * 2 + lh) * 2 * T * 16;
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-          ah[r] = *reinterpret_cast<const f16x8*>(pa + o + r * 512);
-          bh[r] = *reinterpret_cast<const f16x8*>(pb + o + r * 512);
-          al[r] = *reinterpret_cast<const f16x8*>(pa + o + T * 16 + r * 512);
-          bl[r] = *reinterpret_cast<const f16x8*>(pb + o + T * 16 + r * 512);
-        }
-#pragma unroll
-        for (int r = 0; r < R; ++r)
-#pragma unroll
-          for (int c = 0; c < R; ++c) {
-            acc[r][c] = mfma(ah[r], bh[c], acc[r][c]);
-            acx[r][c] = mfma(ah[r], bl[c], acx[r][c]);
-            acx[r][c] = mfma(al[r], bh[c], acx[r][c]);
-          }
+      read(f1, s, 1);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(f0);
+      __builtin_amdgcn_sched_barrier(0);
+      if (s + 1 < n_slots) {
+        enter(s + 1);
+        read(f0, s + 1, 0);
+        __builtin_amdgcn_sched_barrier(0);
       }
+      multiply(f1);
+    }
+    if (partial) {
+      float4* p = reinterpret_cast<float4*>(a.part) + ((long)(idx - a.n_main) * a.split + share) * NQ * 256 + tid;
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int c = 0; c < R; ++c)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = acc[r][c][4 * g + e] + acx[r][c][4 * g + e];
+            p[((r * R + c) * 4 + g) * 256] = make_float4(v[0], v[1], v[2], v[3]);
+          }
+      return;
     }
   }
 
   // Accumulator block: lane (li, lh) holds column li, rows 8 g + 4 lh + v (g, v = 0..3).
   const float da = pow2f(-ea), db = pow2f(-eb), so = pow2f(eo);
-  const int ib = i0 + wm * 32 * R, jb = j0 + wn * 32 * R;
+  const int ib = i0 + wm * 32 * R + (JOIN ? set / R * 32 : 0), jb = j0 + wn * 32 * R + (JOIN ? set % R * 32 : 0);
   if constexpr (KIND == K_OUT) {
     const Hyper h = get_hyper(a.h, a.hyper_dev);
     const float keep = 1.f - h.lr * h.wd, rate = h.lr * j.scale;
+    const int rows = j.rows, cols = j.cols;
+    typedef __attribute__((address_space(1))) float gfloat;
+    gfloat* const p = (gfloat*)(float*)j.dst;
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+    for (int r = 0; r < RA; ++r)
 #pragma unroll
-      for (int c = 0; c < R; ++c) {
-        const int col = jb + c * 32 + li;
-        if (col >= j.cols) continue;
+      for (int c = 0; c < RA; ++c) {
+        const int col = jb + c * 32 + li, row0 = ib + r * 32 + 4 * lh;
+        if (col >= cols) continue;
+        float old[16];
+        if constexpr (DT == 3)          // (all of a block's weights are requested before the first is used)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) {
+            const int row = row0 + 8 * (v >> 2) + (v & 3);
+            old[v] = row < rows ? p[(long)row * cols + col] : 0.f;
+          }
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
-          const int row = ib + r * 32 + 8 * (v >> 2) + 4 * lh + (v & 3);
-          if (row >= j.rows) continue;
+          const int row = row0 + 8 * (v >> 2) + (v & 3);
           const float x = (acc[r][c][v] + acx[r][c][v]) * da * db;
-          const long o = (long)row * j.cols + col;
-          if constexpr (DT == 3) {
-            float* p = reinterpret_cast<float*>(j.dst) + o;
-            *p = fmaf(-rate, x, *p * keep);
-          } else {
-            store1<DT>(j.dst, o, x);
+          const long o = (long)row * cols + col;
+          if (row < rows) {
+            if constexpr (DT == 3) p[o] = fmaf(-rate, x, old[v] * keep);
+            else store1<DT>(j.dst, o, x);
           }
         }
       }
@@ -528,9 +629,9 @@ __global__ __launch_bounds__(256, 2) void orth_gemm_k(GemmArgs a) {
     __syncthreads();                                   // the ring becomes the transposing buffer
     float* tr = reinterpret_cast<float*>(smem) + wave * 32 * 33;
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+    for (int r = 0; r < RA; ++r)
 #pragma unroll
-      for (int c = 0; c < R; ++c) {
+      for (int c = 0; c < RA; ++c) {
         const int rb = ib + r * 32, cb = jb + c * 32;
         // A symmetric product is written once and mirrored: blocks under the diagonal are skipped, a block on it takes its own upper half
         // twice.  (Left as computed, the halves differ by their roundings, and a product with such a matrix is not S^2 but S S^T: from the
@@ -606,9 +707,31 @@ Groups make_groups(int steps, float a, double limit) {
 struct OrthPlan {
   int64_t jobs_b, ew_b, split_b, sym_b, fin_b, head_b, total_b;
   int64_t n_ew, n_split, n_sym, n_fin;
-  int tile;
+  int64_t part_b;
+  int k_gram, k_m, k_fin;        // mean number of K slots of a tile's product: X X^T, m x m products, P X
+  int tile_sym, tile_fin, pad;
   Groups g;
 };
+
+// How a launch of n tiles with k slots each fills the chip.  A CU holds two 128-tiles or three 64-tiles at a time; the tiles left after
+// the full rounds are split along K over the idle places when that saves more than the join costs: over 32 slots of 0.3 us (a lone
+// 64-tile) to 0.7 us, against 7 to 10 us.  1024 x 4096, X X^T (136 tiles, 128 slots): 44 us whole, 31 split in five and joined; at 32
+// slots 13 whole, 17 split.
+struct Fill { int n_main, split; };
+Fill fill_for(int64_t n, int k, int tile) {
+  const int64_t places = 256 * (tile == 128 ? 2 : 3), rest = n % places;
+  Fill f{(int)n, 1};
+  if (rest == 0) return f;
+  int64_t split = places / rest;
+  if (split > k / 4) split = k / 4;
+  if (split > 16) split = 16;
+  if (split >= 2 && k - k / split > 32) { f.n_main = (int)(n - rest); f.split = (int)split; }
+  return f;
+}
+int64_t part_bytes(int64_t n, int k, int tile) {
+  const Fill f = fill_for(n, k, tile);
+  return (n - f.n_main) * f.split * (int64_t)tile * tile * 4;
+}
 
 int make_plan(const mpose_orth_job* jobs, int n_jobs, const mpose_orth_options* o, bool muon, OrthPlan& p) {
   if (n_jobs < 0 || n_jobs > 65535 || !o || (n_jobs > 0 && !jobs)) return MPOSE_EINVAL;
@@ -623,31 +746,67 @@ int make_plan(const mpose_orth_job* jobs, int n_jobs, const mpose_orth_options* 
   }
   p = OrthPlan{};
   p.g = make_groups(o->steps, o->a, muon ? 150.0 : 12.0);
-  p.tile = 64;
-  int64_t body = 0;
+  // Tile sizes: 128 reads half as many operand bytes per product but wants enough tiles to fill the chip, and matrices that it does not pad by
+  // more than an eighth.  4096 x 4096: symmetric products 252 us with 64, 196 with 128, P X 472 and 365; 1024 x 1024 (36 tiles): 13 and 28 us.
+  int64_t area[2][2] = {}, count[2][2] = {};        // [64, 128][symmetric, P X]
   for (int i = 0; i < n_jobs; ++i) {
     const int rows = jobs[i].rows, cols = jobs[i].cols;
     if (rows < 1 || cols < 1 || rows > (1 << 21) || cols > (1 << 21) || (int64_t)rows * cols > (1 << 28)) return MPOSE_EINVAL;
-    const OrthLayout l = orth_layout(rows, cols, p.tile, p.g.n);
+    const int64_t m = rows < cols ? rows : cols;
+    for (int t = 0; t < 2; ++t) {
+      const int64_t T = 64 << t, tm = (m + T - 1) / T, tf = ((rows + T - 1) / T) * ((cols + T - 1) / T);
+      count[t][0] += tm * (tm + 1) / 2; count[t][1] += tf;
+      area[t][0] += tm * tm * T * T; area[t][1] += tf * T * T;
+    }
+  }
+  p.tile_sym = count[1][0] >= 384 && area[1][0] * 8 <= area[0][0] * 9 ? 128 : 64;
+  p.tile_fin = count[1][1] >= 192 && area[1][1] * 8 <= area[0][1] * 9 ? 128 : 64;
+  p.pad = p.tile_sym > p.tile_fin ? p.tile_sym : p.tile_fin;
+  int64_t body = 0, s_gram = 0, s_m = 0, s_fin = 0;
+  for (int i = 0; i < n_jobs; ++i) {
+    const int rows = jobs[i].rows, cols = jobs[i].cols;
+    const OrthLayout l = orth_layout(rows, cols, p.pad, p.g.n);
     body += l.total;
     p.n_ew += l.n_part;
     p.n_split += (int64_t)((rows + 63) / 64) * ((cols + 63) / 64);
-    const int64_t tm = l.mp / p.tile;
-    p.n_sym += tm * (tm + 1) / 2;
-    p.n_fin += (int64_t)(l.rp / p.tile) * (l.cp / p.tile);
+    const int m = rows < cols ? rows : cols;
+    const int64_t tm = (m + p.tile_sym - 1) / p.tile_sym, ns = tm * (tm + 1) / 2;
+    const int64_t nf = (int64_t)((rows + p.tile_fin - 1) / p.tile_fin) * ((cols + p.tile_fin - 1) / p.tile_fin);
+    p.n_sym += ns;
+    p.n_fin += nf;
+    s_gram += ns * ((rows < cols ? l.ck : l.rk) / 32);
+    s_m += ns * (l.mk / 32);
+    s_fin += nf * (l.mk / 32);
   }
+  if (n_jobs > 0) { p.k_gram = (int)(s_gram / p.n_sym); p.k_m = (int)(s_m / p.n_sym); p.k_fin = (int)(s_fin / p.n_fin); }
+  const int64_t parts[4] = {part_bytes(p.n_sym, p.k_gram, p.tile_sym), part_bytes(p.n_sym, p.k_m, p.tile_sym), part_bytes(2 * p.n_sym, p.k_m, p.tile_sym),
+                            part_bytes(p.n_fin, p.k_fin, p.tile_fin)};
+  for (int64_t b : parts) p.part_b = b > p.part_b ? b : p.part_b;
   if (p.n_ew > (1 << 30) || p.n_split > (1 << 30) || p.n_sym > (1 << 30) || p.n_fin > (1 << 30)) return MPOSE_EINVAL;
   auto up = [](int64_t b) { return (b + 255) / 256 * 256; };
   p.jobs_b = up((int64_t)n_jobs * (int64_t)sizeof(OrthJob));
   p.ew_b = up(p.n_ew * 8); p.split_b = up(p.n_split * 8); p.sym_b = up(p.n_sym * 8); p.fin_b = up(p.n_fin * 8);
-  p.head_b = p.jobs_b + p.ew_b + p.split_b + p.sym_b + p.fin_b;
+  p.head_b = p.jobs_b + p.ew_b + p.split_b + p.sym_b + p.fin_b + p.part_b;
   p.total_b = p.head_b + body;
   return 0;
 }
 
+template <int R, int NBUF, int KIND, int DT>
+void gemm_tile(const GemmArgs& a, int64_t n, hipStream_t s) {
+  const unsigned whole = (unsigned)((a.n_main + 7) / 8 * 8), rest = (unsigned)(n - a.n_main);
+  launch(orth_gemm_k<R, NBUF, KIND, DT, false>, dim3(whole + rest * (unsigned)a.split), dim3(256), 0, s, a);
+  if (rest > 0) launch(orth_gemm_k<R, NBUF, KIND, DT, true>, dim3(rest * R * R), dim3(256), 0, s, a);
+}
+
+// One product of every matrix.  k: mean number of K slots; halves: 2 when the launch makes both W and P.
 template <int KIND, int DT = 0>
-void gemm(const GemmArgs& a, int ny, hipStream_t s) {
-  launch(orth_gemm_k<1, 3, KIND, DT>, dim3((unsigned)((a.n_tiles + 7) / 8 * 8), (unsigned)ny), dim3(256), 0, s, a);
+void gemm(GemmArgs a, int tile, int k, int halves, hipStream_t s) {
+  const int64_t n = (int64_t)a.n_tiles * halves;
+  const Fill f = fill_for(n, k, tile);
+  a.n_main = f.n_main; a.split = f.split;
+  if (tile == 128) gemm_tile<2, 2, KIND, DT>(a, n, s);
+  else if (n <= 256 && f.split == 1) gemm_tile<1, 8, KIND, DT>(a, n, s);       // one tile per CU at most: a deep ring instead of neighbours
+  else gemm_tile<1, 3, KIND, DT>(a, n, s);
 }
 
 int run(const mpose_orth_job* jobs, int n_jobs, const mpose_orth_options* o, bool muon, const Hyper& h, const float* hyper_dev, void* ws, int64_t ws_bytes,
@@ -670,19 +829,20 @@ int run(const mpose_orth_job* jobs, int n_jobs, const mpose_orth_options* o, boo
   sa.split = (int2*)base; base += p.split_b;
   sa.sym = (int2*)base; base += p.sym_b;
   sa.fin = (int2*)base; base += p.fin_b;
-  sa.tile = p.tile; sa.n_groups = p.g.n; sa.elem = elem;
+  float* const part = (float*)base; base += p.part_b;
+  sa.pad = p.pad; sa.tile_sym = p.tile_sym; sa.tile_fin = p.tile_fin; sa.n_groups = p.g.n; sa.elem = elem;
   int ew = 0, split = 0, sym = 0, fin = 0;
   for (int i = 0; i < n_jobs; ++i) {
     if (sa.n == 0) sa.first = i;
     SetupJob& j = sa.j[sa.n++];
     j = SetupJob{jobs[i].src, muon ? jobs[i].buf : nullptr, jobs[i].dst, base, jobs[i].rows, jobs[i].cols, jobs[i].scale, ew, split, sym, fin};
-    const OrthLayout l = orth_layout(j.rows, j.cols, p.tile, p.g.n);
+    const OrthLayout l = orth_layout(j.rows, j.cols, p.pad, p.g.n);
     base += l.total;
     ew += l.n_part;
     split += ((j.rows + 63) / 64) * ((j.cols + 63) / 64);
-    const int tm = l.mp / p.tile;
+    const int m = j.rows < j.cols ? j.rows : j.cols, tm = (m + p.tile_sym - 1) / p.tile_sym;
     sym += tm * (tm + 1) / 2;
-    fin += (l.rp / p.tile) * (l.cp / p.tile);
+    fin += ((j.rows + p.tile_fin - 1) / p.tile_fin) * ((j.cols + p.tile_fin - 1) / p.tile_fin);
     if (sa.n == kSetupJobs || i == n_jobs - 1) {
       launch(orth_setup_k, dim3((unsigned)sa.n), dim3(256), 0, s, sa);
       sa.n = 0;
@@ -697,7 +857,7 @@ int run(const mpose_orth_job* jobs, int n_jobs, const mpose_orth_options* o, boo
   else if (o->dtype == 0) launch(orth_norm_k<0, false>, ge, wg, 0, s, pa);
   else if (o->dtype == 1) launch(orth_norm_k<1, false>, ge, wg, 0, s, pa);
   else launch(orth_norm_k<2, false>, ge, wg, 0, s, pa);
-  launch(orth_scalars_k, dim3((unsigned)n_jobs), dim3(64), 0, s, sa.jobs, k, (double)o->eps, o->steps, p.g.mask);
+  launch(orth_scalars_k, dim3((unsigned)n_jobs), dim3(256), 0, s, sa.jobs, k, (double)o->eps, o->steps, p.g.mask);
   pa.list = sa.split;
   if (muon) launch(orth_split_k<0, true>, gs, wg, 0, s, pa);
   else if (o->dtype == 0) launch(orth_split_k<0, false>, gs, wg, 0, s, pa);
@@ -705,27 +865,27 @@ int run(const mpose_orth_job* jobs, int n_jobs, const mpose_orth_options* o, boo
   else launch(orth_split_k<2, false>, gs, wg, 0, s, pa);
 
   GemmArgs ga{};
-  ga.jobs = sa.jobs; ga.k = k; ga.h = h; ga.hyper_dev = hyper_dev;
+  ga.jobs = sa.jobs; ga.k = k; ga.h = h; ga.hyper_dev = hyper_dev; ga.part = part;
   for (int g = 0; g < p.g.n; ++g) {
     ga.step0 = p.g.first[g]; ga.parity = g & 1;
     ga.list = sa.sym; ga.n_tiles = (int)p.n_sym;
     ga.step = ga.step0; ga.i = 0;
-    gemm<K_GRAM>(ga, 1, s);
+    gemm<K_GRAM>(ga, p.tile_sym, p.k_gram, 1, s);
     for (int i = 0; i < p.g.size[g]; ++i) {
       ga.i = i; ga.step = ga.step0 + i;
       const bool last = i == p.g.size[g] - 1;
-      gemm<K_Q>(ga, 1, s);
+      gemm<K_Q>(ga, p.tile_sym, p.k_m, 1, s);
       // W = Q S unless this is the group's last step, P = Q P unless it is its first
       ga.y0 = last ? 1 : 0;
-      if (!last || i > 0) gemm<K_MUL>(ga, (last ? 0 : 1) + (i > 0 ? 1 : 0), s);
-      if (!last) gemm<K_NEXT>(ga, 1, s);
+      if (!last || i > 0) gemm<K_MUL>(ga, p.tile_sym, p.k_m, (last ? 0 : 1) + (i > 0 ? 1 : 0), s);
+      if (!last) gemm<K_NEXT>(ga, p.tile_sym, p.k_m, 1, s);
     }
     ga.list = sa.fin; ga.n_tiles = (int)p.n_fin;
-    if (g + 1 < p.g.n) gemm<K_X>(ga, 1, s);
-    else if (muon) gemm<K_OUT, 3>(ga, 1, s);
-    else if (o->dtype == 0) gemm<K_OUT, 0>(ga, 1, s);
-    else if (o->dtype == 1) gemm<K_OUT, 1>(ga, 1, s);
-    else gemm<K_OUT, 2>(ga, 1, s);
+    if (g + 1 < p.g.n) gemm<K_X>(ga, p.tile_fin, p.k_fin, 1, s);
+    else if (muon) gemm<K_OUT, 3>(ga, p.tile_fin, p.k_fin, 1, s);
+    else if (o->dtype == 0) gemm<K_OUT, 0>(ga, p.tile_fin, p.k_fin, 1, s);
+    else if (o->dtype == 1) gemm<K_OUT, 1>(ga, p.tile_fin, p.k_fin, 1, s);
+    else gemm<K_OUT, 2>(ga, p.tile_fin, p.k_fin, 1, s);
   }
   return launch_status();
 }
