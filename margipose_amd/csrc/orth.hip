@@ -33,6 +33,7 @@ typedef __attribute__((address_space(3))) void* lds_void_p;
 constexpr int kMaxSteps = 24;
 constexpr int kChunk = 4096;            // elements per workgroup of the momentum / norm pass
 constexpr int kSetupJobs = 48;          // jobs per set-up launch (they travel as kernel arguments: 4 KB)
+constexpr int kChainMax = 192;          // largest m whose products run as one chain in one workgroup's LDS
 constexpr float kGrowth = 1024.f;       // largest singular value that a polynomial may make of one in [0, 1]
 
 struct StepExp { int x, s, q, w, p; };  // scale exponents of X (a group's first step), S, Q, W, P
@@ -86,12 +87,14 @@ struct SetupJob {
   unsigned char* ws;
   int rows, cols;
   float scale;
-  int ew0, split0, sym0, fin0;          // where the job's entries start in the lists
+  int ew0, split0, sym0, big0, fin0;    // where the job's entries start in the lists
+  int chain;                            // place in the chain list, or -1: the matrix's m x m products run tile by tile (big0)
 };
 struct SetupArgs {
   SetupJob j[kSetupJobs];
   OrthJob* jobs;
-  int2 *ew, *split, *sym, *fin;
+  int2 *ew, *split, *sym, *big, *fin;
+  int* chain;
   int first, n, pad, tile_sym, tile_fin, n_groups, elem;
 };
 
@@ -124,6 +127,7 @@ __global__ __launch_bounds__(256) void orth_setup_k(SetupArgs a) {
     o->rows = j.rows; o->cols = j.cols; o->m = j.rows < j.cols ? j.rows : j.cols;
     o->mp = l.mp; o->mk = l.mk; o->rp = l.rp; o->cp = l.cp; o->rk = l.rk; o->ck = l.ck;
     o->wide = j.rows <= j.cols;
+    if (j.chain >= 0) a.chain[j.chain] = id;
     const uint64_t bits = (uint64_t)j.src | (uint64_t)j.buf | (uint64_t)j.dst | ((uint64_t)j.cols * (uint64_t)a.elem);
     o->aligned = (bits & (uint64_t)(4 * a.elem - 1)) == 0;        // four elements at a time: every row starts on that boundary
   }
@@ -133,7 +137,10 @@ __global__ __launch_bounds__(256) void orth_setup_k(SetupArgs a) {
   const int m = j.rows < j.cols ? j.rows : j.cols, tm = (m + a.tile_sym - 1) / a.tile_sym;
   for (int i = threadIdx.x; i < tm * tm; i += 256) {
     const int r = i / tm, c = i % tm;
-    if (c >= r) a.sym[j.sym0 + upper_place(r, c, tm)] = make_int2(id, r | (c << 16));
+    if (c < r) continue;
+    const int at = upper_place(r, c, tm);
+    a.sym[j.sym0 + at] = make_int2(id, r | (c << 16));
+    if (j.chain < 0) a.big[j.big0 + at] = make_int2(id, r | (c << 16));
   }
   const int tr = (j.rows + a.tile_fin - 1) / a.tile_fin, tc = (j.cols + a.tile_fin - 1) / a.tile_fin;
   for (int i = threadIdx.x; i < tr * tc; i += 256) {
@@ -468,7 +475,7 @@ __global__ __launch_bounds__(256, NBUF * R > 4 ? 1 : 2) void orth_gemm_k(GemmArg
   } else if constexpr (KIND == K_NEXT) {
     A = j.w; ea = e.w; B = j.q[a.i & 1]; eb = e.q; eo = j.e[a.step + 1].s; out = j.s;
   } else {
-    const unsigned char* P = a.i == 0 ? j.q[0] : j.p[a.i & 1];
+    const unsigned char* P = a.i == 0 && j.m > kChainMax ? j.q[0] : j.p[j.m > kChainMax ? a.i & 1 : 0];
     const unsigned char* X = j.wide ? j.t[a.parity] : j.n[a.parity];
     A = j.wide ? P : X; B = j.wide ? X : P;
     arp = j.rp; brp = j.cp;
@@ -685,6 +692,240 @@ __global__ __launch_bounds__(256, NBUF * R > 4 ? 1 : 2) void orth_gemm_k(GemmArg
   }
 }
 
+// ---- the m x m products of one group as one chain, one workgroup per matrix (m <= 192) ----
+// Launched product by product, a model's few hundred 192 x 192 matrices pass through the Infinity Cache at each of them (120 MB a launch: 25 us
+// each, 14 launches).  Here S, then Q, sits in LDS (147 KB at m = 192) as the left operand, and a wave holds 16 columns of the right
+// operand and of the result in registers: the result of one product is the right operand of the next without moving.  For that the K axis
+// of a k = 32 step is permuted alike on both sides: element 4 t + v of lane quarter q is k = 32 s + 16 t + 4 q + v, which is where the
+// 16 x 16 accumulators have their rows (4 q + v).  What goes to LDS is the result's transpose (8 bytes a store): with L = M^T there,
+// Q = q(S^T S), W = S^T Q, P <- Q^T P and S <- Q^T W stay symmetric up to one product's rounding (no loss measured).
+// P waits in memory between its products (private to the wave).  16 columns, not 32: with 32 x 32 blocks two panels of 192 rows, the
+// accumulators and the fragments do not fit the 256 registers of a wave.
+struct ChainArgs {
+  const OrthJob* jobs;
+  const int* list;
+  int step0, size;
+  Poly k;
+};
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+template <int NS>                                            // NS = mk / 32: K steps of a product, half its waves and row blocks
+struct Panel { f16x8 h[NS], l[NS]; };
+
+__device__ __forceinline__ f16x4 half8(const f16x8 a, int t) { return t ? __builtin_shufflevector(a, a, 4, 5, 6, 7) : __builtin_shufflevector(a, a, 0, 1, 2, 3); }
+
+// In LDS: [step of 32][plane][lane quarter][row][16 B]: a fragment is one ds_read_b128, a result one ds_write_b128 (with the octets of H8
+// a fragment is two pieces of 8 bytes: 64 B per clock).  Three lane addresses, 48 KB apart at m = 192: every other offset is an immediate.
+typedef __attribute__((address_space(3))) unsigned char lds_byte;
+typedef __attribute__((address_space(3))) f16x8 lds_f16x8;
+template <int NS>
+struct LdsBase { lds_byte* p[(NS + 1) / 2]; };
+template <int NS>
+__device__ __forceinline__ lds_f16x8* chain_at(const LdsBase<NS>& b, int s, int plane, int rb) {
+  constexpr int RL = 32 * NS;
+  return (lds_f16x8*)(b.p[s >> 1] + (((s & 1) * 2 + plane) * 4 * RL + rb * 16) * 16);
+}
+template <int NS>
+__device__ __forceinline__ LdsBase<NS> chain_base(unsigned char* lds, int row, int lq) {
+  LdsBase<NS> b;
+#pragma unroll
+  for (int k = 0; k < (NS + 1) / 2; ++k) {
+    b.p[k] = (lds_byte*)lds + ((k * 16 + lq) * 32 * NS + row) * 16;
+    asm volatile("" : "+v"(b.p[k]));
+  }
+  return b;
+}
+
+// rows 16 rb .. of L times the panel; `a`: the lane's row, octet and half
+template <int NS>
+__device__ __forceinline__ f32x4 chain_rows(const LdsBase<NS>& a, const Panel<NS>& b, int rb) {
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f}, acx = acc;
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    const f16x8 h = *chain_at<NS>(a, s, 0, rb), l = *chain_at<NS>(a, s, 1, rb);
+    acx = __builtin_amdgcn_mfma_f32_16x16x32_f16(h, b.l[s], acx, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(h, b.h[s], acc, 0, 0, 0);
+    acx = __builtin_amdgcn_mfma_f32_16x16x32_f16(l, b.h[s], acx, 0, 0, 0);
+  }
+  asm volatile("" ::: "memory");      // (the next product over the same rows reads them again: kept from here they would spill)
+  return acc + acx;
+}
+
+// two row blocks of results -> one K step of a panel (whole registers at a time: element by element the halves are kept apart)
+__device__ __forceinline__ void chain_pack(const f32x4 x0, const f32x4 x1, f16x8& h, f16x8& l) {
+  f16x8 hh, ll;
+#pragma unroll
+  for (int v = 0; v < 4; ++v) {
+    _Float16 p, q;
+    split16(x0[v], p, q);
+    hh[v] = p; ll[v] = q;
+    split16(x1[v], p, q);
+    hh[4 + v] = p; ll[4 + v] = q;
+  }
+  u32x4 hu, lu;
+  __builtin_memcpy(&hu, &hh, 16);
+  __builtin_memcpy(&lu, &ll, 16);
+  asm volatile("" : "+v"(hu), "+v"(lu));
+  __builtin_memcpy(&h, &hu, 16);
+  __builtin_memcpy(&l, &lu, 16);
+}
+
+// one K step of a panel's transpose as H8 in memory: row = the panel's column, octets = its rows
+__device__ __forceinline__ void chain_store(unsigned char* base, unsigned off, unsigned ld, int s, const f16x8 h, const f16x8 l) {
+  typedef __attribute__((address_space(1))) unsigned char glob_byte;
+  typedef __attribute__((address_space(1))) f16x4 glob_f16x4;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const unsigned o = off + (unsigned)(8 * s + 4 * t) * ld * 16u;
+    *(glob_f16x4*)((glob_byte*)base + o) = half8(h, t);
+    *(glob_f16x4*)((glob_byte*)base + o + ld * 16u) = half8(l, t);
+  }
+}
+
+template <int NS>
+__device__ __forceinline__ void chain_fill(const LdsBase<NS>& d, const Panel<NS>& b) {
+#pragma unroll
+  for (int s = 0; s < NS; ++s) { *chain_at<NS>(d, s, 0, 0) = b.h[s]; *chain_at<NS>(d, s, 1, 0) = b.l[s]; }
+}
+
+template <int NS>
+__device__ __forceinline__ void orth_chain(const OrthJob& j, const ChainArgs& a, unsigned char* lds) {
+  constexpr int RL = 32 * NS, NB = 2 * NS;                   // rows in LDS; row blocks = waves
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 15, lq = lane >> 4;
+  const bool on = w < NB;
+  const int m = j.m, mp = j.mp, col = on ? w * 16 + li : 0;
+  // S into LDS, its padding cleared
+  for (int i = tid; i < 8 * NS * RL; i += (int)blockDim.x) {
+    const int row = i % RL, slab = i / RL;
+    u32x4 v = {0u, 0u, 0u, 0u};
+    if (row < m) v = *reinterpret_cast<const u32x4*>(j.s + ((long)slab * mp + row) * 16);
+    // global: [octet][plane]; the octet's halves belong to two lane quarters, as their piece t
+    const int oct = slab >> 1, t = (oct >> 1) & 1, lq0 = (oct & 1) * 2;
+    unsigned char* d = lds + ((((oct >> 2) * 2 + (slab & 1)) * 4 + lq0) * RL + row) * 16 + t * 8;
+    *reinterpret_cast<uint2*>(d) = make_uint2(v[0], v[1]);
+    *reinterpret_cast<uint2*>(d + RL * 16) = make_uint2(v[2], v[3]);
+  }
+  __syncthreads();
+  Panel<NS> cur, out;
+  if (on) {
+    const LdsBase<NS> lw = chain_base<NS>(lds, col, lq);
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      cur.h[s] = *chain_at<NS>(lw, s, 0, 0);
+      cur.l[s] = *chain_at<NS>(lw, s, 1, 0);
+    }
+  }
+  for (int i = 0; i < a.size; ++i) {
+    const StepExp e = j.e[a.step0 + i];
+    const bool last = i == a.size - 1;
+    // (opaque to the compiler: it would keep the 48 comparisons and store addresses made from them in registers over the whole loop)
+    int c = col - 4 * lq, ld = mp, zero = 0;
+    asm volatile("" : "+v"(c), "+v"(ld), "+v"(zero));
+    typedef __attribute__((address_space(1))) f16x8 glob_f16x8;
+    const unsigned mine = (unsigned)(w * 2 * NS * 64 + lane + zero);
+    glob_f16x8* const keep = (glob_f16x8*)(f16x8*)j.p[1] + mine;
+    glob_f16x8* const park = (glob_f16x8*)(f16x8*)j.w + mine;
+    const LdsBase<NS> la = chain_base<NS>(lds, li, lq);
+    if (on) {                                  // out = Q
+      const float ds = pow2f(-e.s), so = pow2f(e.q), a_diag = col < m ? a.k.a : 0.f;
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        f32x4 x[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          x[t] = chain_rows<NS>(la, cur, 2 * s + t);
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const float sv = ((float)cur.h[s][4 * t + v] + (float)cur.l[s][4 * t + v]) * ds;
+            x[t][v] = (fmaf(a.k.c, x[t][v] * ds * ds, a.k.b * sv) + (c == s * 32 + t * 16 + v ? a_diag : 0.f)) * so;
+          }
+        }
+        chain_pack(x[0], x[1], out.h[s], out.l[s]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (!last) {                             // cur = W = S Q
+        const float dw = pow2f(-e.q) * pow2f(e.w);
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+          const f32x4 x0 = chain_rows<NS>(la, out, 2 * s) * ds * dw, x1 = chain_rows<NS>(la, out, 2 * s + 1) * ds * dw;
+          chain_pack(x0, x1, cur.h[s], cur.l[s]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    }
+    if (last && i == 0) {                      // a group of one step: P = Q
+      if (on) {
+        const unsigned off = (unsigned)((c + 4 * lq) * 16 + (lq >> 1) * 2 * ld * 16 + (lq & 1) * 8);
+#pragma unroll
+        for (int s = 0; s < NS; ++s) chain_store(j.p[0], off, (unsigned)ld, s, out.h[s], out.l[s]);
+      }
+      break;
+    }
+    __syncthreads();                           // every wave has read S
+    if (on) {
+      chain_fill<NS>(chain_base<NS>(lds, c + 4 * lq, lq), out);
+      if (i == 0) {
+#pragma unroll
+        for (int s = 0; s < NS; ++s) { keep[(2 * s) * 64] = out.h[s]; keep[(2 * s + 1) * 64] = out.l[s]; }
+      }
+    }
+    __syncthreads();                           // Q is whole
+    constexpr bool kPark = NS > 4;             // two panels and P's results do not fit the registers there: W waits in memory too
+    if (on && i > 0) {                         // P <- Q P
+      if (kPark) {
+#pragma unroll
+        for (int s = 0; s < NS; ++s) { park[(2 * s) * 64] = cur.h[s]; park[(2 * s + 1) * 64] = cur.l[s]; }
+      }
+      const float dp = pow2f(-j.e[a.step0 + i - 1].p), dq = pow2f(-e.q) * pow2f(e.p);
+#pragma unroll
+      for (int s = 0; s < NS; ++s) { out.h[s] = keep[(2 * s) * 64]; out.l[s] = keep[(2 * s + 1) * 64]; }
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        f16x8 h, l;
+        const f32x4 x0 = chain_rows<NS>(la, out, 2 * s) * dp * dq, x1 = chain_rows<NS>(la, out, 2 * s + 1) * dp * dq;
+        chain_pack(x0, x1, h, l);
+        if (last) {
+          chain_store(j.p[0], (unsigned)((c + 4 * lq) * 16 + (lq >> 1) * 2 * ld * 16 + (lq & 1) * 8), (unsigned)ld, s, h, l);
+        } else {
+          keep[(2 * s) * 64] = h; keep[(2 * s + 1) * 64] = l;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (kPark) {
+#pragma unroll
+        for (int s = 0; s < NS; ++s) { cur.h[s] = park[(2 * s) * 64]; cur.l[s] = park[(2 * s + 1) * 64]; }
+      }
+    }
+    if (last) break;
+    if (on) {                                  // S <- Q W
+      const float dq = pow2f(-e.q), dw = pow2f(-e.w) * pow2f(j.e[a.step0 + i + 1].s);
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        const f32x4 x0 = chain_rows<NS>(la, cur, 2 * s) * dq * dw, x1 = chain_rows<NS>(la, cur, 2 * s + 1) * dq * dw;
+        chain_pack(x0, x1, out.h[s], out.l[s]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    __syncthreads();                           // every wave has read Q
+    if (on) { chain_fill<NS>(chain_base<NS>(lds, c + 4 * lq, lq), out); cur = out; }
+    __syncthreads();
+  }
+}
+
+__global__ __launch_bounds__(128 * (kChainMax / 32)) void orth_chain_k(ChainArgs a) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char chain_lds[];
+  const OrthJob& j = a.jobs[a.list[blockIdx.x]];
+  switch (j.mk / 32) {
+    case 1: orth_chain<1>(j, a, chain_lds); break;
+    case 2: orth_chain<2>(j, a, chain_lds); break;
+    case 3: orth_chain<3>(j, a, chain_lds); break;
+    case 4: orth_chain<4>(j, a, chain_lds); break;
+    case 5: orth_chain<5>(j, a, chain_lds); break;
+    default: orth_chain<6>(j, a, chain_lds); break;
+  }
+}
+
 // ---- host ----
 struct Groups { int n, first[kMaxSteps], size[kMaxSteps], mask; };
 
@@ -705,8 +946,9 @@ Groups make_groups(int steps, float a, double limit) {
 }
 
 struct OrthPlan {
-  int64_t jobs_b, ew_b, split_b, sym_b, fin_b, head_b, total_b;
-  int64_t n_ew, n_split, n_sym, n_fin;
+  int64_t jobs_b, ew_b, split_b, sym_b, big_b, fin_b, chain_b, head_b, total_b;
+  int64_t n_ew, n_split, n_sym, n_big, n_fin;
+  int n_chain[kChainMax / 32 + 1];        // chained matrices by mk / 32
   int64_t part_b;
   int k_gram, k_m, k_fin;        // mean number of K slots of a tile's product: X X^T, m x m products, P X
   int tile_sym, tile_fin, pad;
@@ -773,20 +1015,21 @@ int make_plan(const mpose_orth_job* jobs, int n_jobs, const mpose_orth_options* 
     const int64_t tm = (m + p.tile_sym - 1) / p.tile_sym, ns = tm * (tm + 1) / 2;
     const int64_t nf = (int64_t)((rows + p.tile_fin - 1) / p.tile_fin) * ((cols + p.tile_fin - 1) / p.tile_fin);
     p.n_sym += ns;
+    if (m <= kChainMax) p.n_chain[l.mk / 32] += 1;
+    else { p.n_big += ns; s_m += ns * (l.mk / 32); }
     p.n_fin += nf;
     s_gram += ns * ((rows < cols ? l.ck : l.rk) / 32);
-    s_m += ns * (l.mk / 32);
     s_fin += nf * (l.mk / 32);
   }
-  if (n_jobs > 0) { p.k_gram = (int)(s_gram / p.n_sym); p.k_m = (int)(s_m / p.n_sym); p.k_fin = (int)(s_fin / p.n_fin); }
-  const int64_t parts[4] = {part_bytes(p.n_sym, p.k_gram, p.tile_sym), part_bytes(p.n_sym, p.k_m, p.tile_sym), part_bytes(2 * p.n_sym, p.k_m, p.tile_sym),
+  if (n_jobs > 0) { p.k_gram = (int)(s_gram / p.n_sym); p.k_m = p.n_big ? (int)(s_m / p.n_big) : 0; p.k_fin = (int)(s_fin / p.n_fin); }
+  const int64_t parts[4] = {part_bytes(p.n_sym, p.k_gram, p.tile_sym), part_bytes(p.n_big, p.k_m, p.tile_sym), part_bytes(2 * p.n_big, p.k_m, p.tile_sym),
                             part_bytes(p.n_fin, p.k_fin, p.tile_fin)};
   for (int64_t b : parts) p.part_b = b > p.part_b ? b : p.part_b;
   if (p.n_ew > (1 << 30) || p.n_split > (1 << 30) || p.n_sym > (1 << 30) || p.n_fin > (1 << 30)) return MPOSE_EINVAL;
   auto up = [](int64_t b) { return (b + 255) / 256 * 256; };
   p.jobs_b = up((int64_t)n_jobs * (int64_t)sizeof(OrthJob));
-  p.ew_b = up(p.n_ew * 8); p.split_b = up(p.n_split * 8); p.sym_b = up(p.n_sym * 8); p.fin_b = up(p.n_fin * 8);
-  p.head_b = p.jobs_b + p.ew_b + p.split_b + p.sym_b + p.fin_b + p.part_b;
+  p.ew_b = up(p.n_ew * 8); p.split_b = up(p.n_split * 8); p.sym_b = up(p.n_sym * 8); p.fin_b = up(p.n_fin * 8); p.big_b = up(p.n_big * 8); p.chain_b = up((int64_t)n_jobs * 4);
+  p.head_b = p.jobs_b + p.ew_b + p.split_b + p.sym_b + p.big_b + p.fin_b + p.chain_b + p.part_b;
   p.total_b = p.head_b + body;
   return 0;
 }
@@ -828,20 +1071,30 @@ int run(const mpose_orth_job* jobs, int n_jobs, const mpose_orth_options* o, boo
   sa.ew = (int2*)base; base += p.ew_b;
   sa.split = (int2*)base; base += p.split_b;
   sa.sym = (int2*)base; base += p.sym_b;
+  sa.big = (int2*)base; base += p.big_b;
+  sa.chain = (int*)base; base += p.chain_b;
   sa.fin = (int2*)base; base += p.fin_b;
   float* const part = (float*)base; base += p.part_b;
   sa.pad = p.pad; sa.tile_sym = p.tile_sym; sa.tile_fin = p.tile_fin; sa.n_groups = p.g.n; sa.elem = elem;
-  int ew = 0, split = 0, sym = 0, fin = 0;
+  int ew = 0, split = 0, sym = 0, big = 0, fin = 0;
+  int chain[kChainMax / 32 + 2] = {}, n_chain = 0, most = 0;      // the longest chains first
+  for (int c = kChainMax / 32; c > 0; --c) {
+    chain[c] = n_chain;
+    n_chain += p.n_chain[c];
+    if (p.n_chain[c] > 0 && most == 0) most = c;
+  }
   for (int i = 0; i < n_jobs; ++i) {
     if (sa.n == 0) sa.first = i;
     SetupJob& j = sa.j[sa.n++];
-    j = SetupJob{jobs[i].src, muon ? jobs[i].buf : nullptr, jobs[i].dst, base, jobs[i].rows, jobs[i].cols, jobs[i].scale, ew, split, sym, fin};
+    j = SetupJob{jobs[i].src, muon ? jobs[i].buf : nullptr, jobs[i].dst, base, jobs[i].rows, jobs[i].cols, jobs[i].scale, ew, split, sym, big, fin, -1};
     const OrthLayout l = orth_layout(j.rows, j.cols, p.pad, p.g.n);
     base += l.total;
     ew += l.n_part;
     split += ((j.rows + 63) / 64) * ((j.cols + 63) / 64);
     const int m = j.rows < j.cols ? j.rows : j.cols, tm = (m + p.tile_sym - 1) / p.tile_sym;
     sym += tm * (tm + 1) / 2;
+    if (m <= kChainMax) j.chain = chain[l.mk / 32]++;
+    else big += tm * (tm + 1) / 2;
     fin += ((j.rows + p.tile_fin - 1) / p.tile_fin) * ((j.cols + p.tile_fin - 1) / p.tile_fin);
     if (sa.n == kSetupJobs || i == n_jobs - 1) {
       launch(orth_setup_k, dim3((unsigned)sa.n), dim3(256), 0, s, sa);
@@ -866,13 +1119,26 @@ int run(const mpose_orth_job* jobs, int n_jobs, const mpose_orth_options* o, boo
 
   GemmArgs ga{};
   ga.jobs = sa.jobs; ga.k = k; ga.h = h; ga.hyper_dev = hyper_dev; ga.part = part;
+  const int chain_lds = most * most * 32 * 32 * 4;
+  if (n_chain > 0) {
+    static bool attr_set = false;          // > 64 KiB of dynamic LDS has to be requested once per kernel
+    if (!attr_set) {
+      if (hipFuncSetAttribute(reinterpret_cast<const void*>(&orth_chain_k), hipFuncAttributeMaxDynamicSharedMemorySize, kChainMax * kChainMax * 4) != hipSuccess)
+        return MPOSE_EINVAL;
+      attr_set = true;
+    }
+  }
   for (int g = 0; g < p.g.n; ++g) {
     ga.step0 = p.g.first[g]; ga.parity = g & 1;
     ga.list = sa.sym; ga.n_tiles = (int)p.n_sym;
     ga.step = ga.step0; ga.i = 0;
     gemm<K_GRAM>(ga, p.tile_sym, p.k_gram, 1, s);
+    if (n_chain > 0)
+      launch(orth_chain_k, dim3((unsigned)n_chain), dim3(128u * (unsigned)most), (size_t)chain_lds, s, ChainArgs{sa.jobs, sa.chain, ga.step0, p.g.size[g], k});
+    ga.list = sa.big; ga.n_tiles = (int)p.n_big;
     for (int i = 0; i < p.g.size[g]; ++i) {
       ga.i = i; ga.step = ga.step0 + i;
+      if (p.n_big == 0) continue;
       const bool last = i == p.g.size[g] - 1;
       gemm<K_Q>(ga, p.tile_sym, p.k_m, 1, s);
       // W = Q S unless this is the group's last step, P = Q P unless it is its first
