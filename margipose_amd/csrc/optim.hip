@@ -70,12 +70,12 @@ extern "C" int mpose_sgd_step(const mpose_sgd_job* jobs_dev, int n_jobs, int64_t
 
 // ---- AdamW ----
 // m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;  p = p (1 - lr wd) - lr c1 m / (sqrt(v) c2 + eps): 28 bytes per element and one pass, so
-// the rate of a large copy bounds it.  The arrays' addresses travel as kernel arguments, 96 arrays a launch (a table in device
+// the rate of a large copy bounds it.  The arrays' addresses travel as kernel arguments, 384 arrays a launch (a table in device
 // memory would need an upload whenever a gradient moves, and could not be captured).
 namespace mpose {
 namespace {
 
-constexpr int kAdamJobs = 96;
+constexpr int kAdamJobs = 384;
 constexpr int kAdamChunk = 4096;
 struct AdamArgs {
   mpose_adamw_job j[kAdamJobs];

@@ -393,7 +393,7 @@ class _DeviceStep:
 
 
 class DeviceAdamW(_DeviceStep):
-    """torch.optim.AdamW's update (decoupled weight decay, no amsgrad) over all parameters as launches of csrc/optim.hip, 96 arrays
+    """torch.optim.AdamW's update (decoupled weight decay, no amsgrad) over all parameters as launches of csrc/optim.hip, 384 arrays
     each:  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2;  p = p (1 - lr wd) - lr m^ / (sqrt(v^) + eps).
     Duck-types DeviceSGD: works in training_step, GraphedTrainStep and PlannedTrainStep, and under make_1cycle -- the schedule's
     `momentum` is beta1.  The moments are two flat arenas (exp_avg_arena, exp_avg_sq_arena), a parameter every 16 bytes."""
