@@ -5,7 +5,7 @@
 //
 // Bound by memory: forward reads x and writes y, backward reads x and dy and writes dx.  So a row is read once and held in registers
 // (E elements of it per thread) between the two reductions and the result: one wave per row up to 1024 columns, a workgroup of 4 or 8
-// waves up to 16384 (8192 where elements are loaded one by one: their addresses take the registers); wider rows are read again from the cache (ln_*_wide_k).  Workgroups walk over the rows with a fixed mapping of columns to
+// waves up to 16384 (8192 backward, and where elements are loaded one by one: registers); wider rows are read again from the cache (ln_*_wide_k).  Workgroups walk over the rows with a fixed mapping of columns to
 // threads, which keeps w and b -- and in the backward pass the running sums of dw and db -- in registers too: one partial row of
 // sums per workgroup goes to memory, a second launch adds the partial rows in a fixed order (no atomics: the same bits every run).
 #include "common.h"
@@ -38,27 +38,42 @@ __device__ __forceinline__ float get_w(const void* p, int dt, int64_t i) {
   return dt == 0 ? get1<0>(p, i) : dt == 1 ? get1<1>(p, i) : get1<2>(p, i);
 }
 
-// V consecutive elements (aligned to their own size)
-template <int DT, int V> __device__ __forceinline__ void getv(const void* p, int64_t i, float* v) {
+// V consecutive elements (aligned to their own size), as they are in memory -- the next row's wait in this form -- and as floats
+template <int DT, int V> struct Raw { unsigned u[V == 1 ? 1 : V * (DT == 0 ? 4 : 2) / 4]; };
+template <int DT, int V> __device__ __forceinline__ void fetch(Raw<DT, V>& r, const void* p, int64_t i) {
   if constexpr (V == 1) {
-    v[0] = get1<DT>(p, i);
-  } else if constexpr (DT == 0) {
-#pragma unroll
-    for (int q = 0; q < V / 4; ++q) {
-      const float4 f = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i + 4 * q);
-      v[4 * q] = f.x; v[4 * q + 1] = f.y; v[4 * q + 2] = f.z; v[4 * q + 3] = f.w;
-    }
+    if constexpr (DT == 0) r.u[0] = reinterpret_cast<const unsigned*>(p)[i];
+    else r.u[0] = reinterpret_cast<const unsigned short*>(p)[i];
   } else {
-    unsigned u[V / 2];
-    if constexpr (V == 4) { const uint2 t = *reinterpret_cast<const uint2*>(reinterpret_cast<const unsigned short*>(p) + i); u[0] = t.x; u[1] = t.y; }
-    else { const uint4 t = *reinterpret_cast<const uint4*>(reinterpret_cast<const unsigned short*>(p) + i); u[0] = t.x; u[1] = t.y; u[2] = t.z; u[3] = t.w; }
+    constexpr int n = V * (DT == 0 ? 4 : 2) / 4;
+    const unsigned char* q = reinterpret_cast<const unsigned char*>(p) + i * (DT == 0 ? 4 : 2);
+    if constexpr (n == 2) {
+      const uint2 t = *reinterpret_cast<const uint2*>(q);
+      r.u[0] = t.x; r.u[1] = t.y;
+    } else {
 #pragma unroll
-    for (int q = 0; q < V / 2; ++q) {
-      if constexpr (DT == 1) { v[2 * q] = __uint_as_float(u[q] << 16); v[2 * q + 1] = __uint_as_float(u[q] & 0xffff0000u); }
-      else {
+      for (int k = 0; k < n / 4; ++k) {
+        const uint4 t = reinterpret_cast<const uint4*>(q)[k];
+        r.u[4 * k] = t.x; r.u[4 * k + 1] = t.y; r.u[4 * k + 2] = t.z; r.u[4 * k + 3] = t.w;
+      }
+    }
+  }
+}
+template <int DT, int V> __device__ __forceinline__ void unpack(const Raw<DT, V>& r, float* v) {
+  if constexpr (DT == 0) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] = __uint_as_float(r.u[k]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < (V + 1) / 2; ++k) {
+      if constexpr (DT == 1) {
+        v[2 * k] = __uint_as_float(r.u[k] << 16);
+        if constexpr (V > 1) v[2 * k + 1] = __uint_as_float(r.u[k] & 0xffff0000u);
+      } else {
         _Float16 h[2];
-        __builtin_memcpy(h, &u[q], 4);
-        v[2 * q] = (float)h[0]; v[2 * q + 1] = (float)h[1];
+        __builtin_memcpy(h, &r.u[k], 4);
+        v[2 * k] = (float)h[0];
+        if constexpr (V > 1) v[2 * k + 1] = (float)h[1];
       }
     }
   }
@@ -139,18 +154,27 @@ __global__ __launch_bounds__(T > 256 ? T : 256) void ln_fwd_k(FwdArgs a) {
       w[i * V + e] = a.w != nullptr && c < cols ? get_w(a.w, a.w_dt, c) : 1.f;
       b[i * V + e] = a.b != nullptr && c < cols ? get_w(a.b, a.w_dt, c) : 0.f;
     }
-  for (int64_t r = (int64_t)blockIdx.x * RW + (T == 64 ? (threadIdx.x >> 6) : 0); r < a.rows; r += (int64_t)gridDim.x * RW) {
-    const int64_t xo = r * a.x_ld;
+  // (the next row's loads are on their way while this row is reduced and written)
+  const int64_t step = (int64_t)gridDim.x * RW;
+  int64_t r = (int64_t)blockIdx.x * RW + (T == 64 ? (threadIdx.x >> 6) : 0);
+  Raw<DT, V> raw[NV];
+  auto ask = [&](int64_t row) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if ((i * T + t) * V < cols) fetch<DT, V>(raw[i], a.x, row * a.x_ld + (i * T + t) * V);
+  };
+  if (r < a.rows) ask(r);
+  for (; r < a.rows; r += step) {
     float x[E];
     float s[1] = {0.f};
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * T + t) * V;
-      if (c < cols) getv<DT, V>(a.x, xo + c, x + i * V);
+      if ((i * T + t) * V < cols) unpack<DT, V>(raw[i], x + i * V);
       else
 #pragma unroll
         for (int e = 0; e < V; ++e) x[i * V + e] = 0.f;
     }
+    if (r + step < a.rows) ask(r + step);
 #pragma unroll
     for (int i = 0; i < E; ++i) s[0] += x[i];
     row_sum<T>(s, sh[0]);
@@ -197,19 +221,31 @@ __global__ __launch_bounds__(T > 256 ? T : 256) void ln_bwd_k(BwdArgs a) {
       dw[i * V + e] = 0.f; db[i * V + e] = 0.f;
     }
   int turn = 0;
-  for (int64_t r = (int64_t)blockIdx.x * RW + (T == 64 ? (threadIdx.x >> 6) : 0); r < a.rows; r += (int64_t)gridDim.x * RW, turn ^= 1) {
-    const int64_t xo = r * a.x_ld, go = r * a.dy_ld;
-    const float mean = a.mean[r], rstd = a.rstd[r];
+  const int64_t step = (int64_t)gridDim.x * RW;
+  int64_t r = (int64_t)blockIdx.x * RW + (T == 64 ? (threadIdx.x >> 6) : 0);
+  Raw<DT, V> rx[NV], rg[NV];
+  float next_mean = 0.f, next_rstd = 0.f;
+  auto ask = [&](int64_t row) {
+    next_mean = a.mean[row]; next_rstd = a.rstd[row];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * T + t) * V;
+      if (c < cols) { fetch<DT, V>(rx[i], a.x, row * a.x_ld + c); fetch<DT, V>(rg[i], a.dy, row * a.dy_ld + c); }
+    }
+  };
+  if (r < a.rows) ask(r);
+  for (; r < a.rows; r += step, turn ^= 1) {
+    const float mean = next_mean, rstd = next_rstd;
     float x[E], g[E];
     float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * T + t) * V;
-      if (c < cols) { getv<DT, V>(a.x, xo + c, x + i * V); getv<DT, V>(a.dy, go + c, g + i * V); }
+      if ((i * T + t) * V < cols) { unpack<DT, V>(rx[i], x + i * V); unpack<DT, V>(rg[i], g + i * V); }
       else
 #pragma unroll
         for (int e = 0; e < V; ++e) { x[i * V + e] = mean; g[i * V + e] = 0.f; }
     }
+    if (r + step < a.rows) ask(r + step);
 #pragma unroll
     for (int i = 0; i < E; ++i) {
       x[i] = (x[i] - mean) * rstd;
@@ -366,7 +402,7 @@ unsigned grid_for(int64_t items, unsigned cap) { return (unsigned)(items < (int6
 template <int DT, int T, int E>
 void fwd_t(const FwdArgs& a, bool vec, hipStream_t s) {
   constexpr int V = E < 16 / (DT == 0 ? 4 : 2) ? E : 16 / (DT == 0 ? 4 : 2);
-  const dim3 grid(grid_for(T == 64 ? (a.rows + 3) / 4 : a.rows, T > 256 ? 512 : 2048)), wg(T > 256 ? T : 256);
+  const dim3 grid(grid_for(T == 64 ? (a.rows + 3) / 4 : a.rows, T > 256 ? 512 : T == 256 ? 1024 : 2048)), wg(T > 256 ? T : 256);
   if (vec) launch(ln_fwd_k<DT, T, E, V>, grid, wg, 0, s, a);
   else if constexpr (E < 32) launch(ln_fwd_k<DT, T, E, 1>, grid, wg, 0, s, a);
 }
@@ -395,8 +431,7 @@ void bwd(const BwdArgs& a, bool vec, hipStream_t s) {
   else if (a.cols <= 1024) bwd_t<DT, 64, 16>(a, vec, s);
   else if (a.cols <= 2048) bwd_t<DT, 256, 8>(a, vec, s);
   else if (a.cols <= 4096) bwd_t<DT, 256, 16>(a, vec, s);
-  else if (a.cols <= 8192) bwd_t<DT, 512, 16>(a, vec, s);
-  else if (a.cols <= kWide && vec) bwd_t<DT, 512, 32>(a, vec, s);
+  else if (a.cols <= kWide / 2) bwd_t<DT, 512, 16>(a, vec, s);
   else {
     if (a.dx != nullptr) launch(ln_bwd_wide_k<DT>, dim3(grid_for(a.rows, 512)), dim3(1024), 0, s, a);
     if (a.part != nullptr) launch(ln_sums_wide_k<DT>, dim3((unsigned)((a.cols + 255) / 256), (unsigned)part_rows(a.rows, a.cols)), dim3(256), 0, s, a);
