@@ -7,9 +7,10 @@
 //     S = X X^T;   per step: Q = q(S), W = Q S, S <- W Q, P <- Q P;   X <- P X,
 // and every m x m product computes only the tiles on and above the diagonal (the others are their transposes).
 // In a group the rounding of S is lifted by a^2 a step where s is small, so a group is as long as a^2 to the power (length - 1) stays below
-// a limit: 12 for mpose_orthogonalize (groups of 2, 2, 1 for the customary a = 3.4445), 150 for mpose_muon_step (3, 2), whose result is
-// a small part of a weight.  Relative error against float64, 128 x 1152, decaying singular values: one group of five 1e-4, (3, 2)
-// 3.4e-6, (2, 2, 1) as X on every step in fp32, 1.4e-6.  Visits of the long axis: 2 against 3.
+// a limit (kLift): 1 for mpose_orthogonalize's fp32 results (X on every step for the customary a = 3.4445), 12 for 16-bit results (groups of
+// 2, 2, 1: their rounding hides the difference), 150 for mpose_muon_step (3, 2), whose result is a small part of a weight.  Relative error
+// against float64, fp32 result: 17 x 128 1.2e-6, 2.0e-6 and 2.4e-6; 128 x 1152 1.1e-6, 1.4e-6 and 3.4e-6 (X on every step in plain fp32:
+// 1.1e-6, 1.4e-6); one group of five 1e-4.  Visits of the long axis: 5, 3, 2.
 //
 // Arithmetic: like the convolutions (three fp16 products of two-way split operands, x * 2^k = h + l: 22 bits), but the scale
 // exponents come from a bound, not from a measurement: |x_ij| <= |X|_2, and a scalar recursion bounds |X|_2, |S|_2, |Q|_2 from the
@@ -33,7 +34,11 @@ typedef __attribute__((address_space(3))) void* lds_void_p;
 constexpr int kMaxSteps = 24;
 constexpr int kChunk = 4096;            // elements per workgroup of the momentum / norm pass
 constexpr int kSetupJobs = 160;         // jobs per set-up launch (they travel as kernel arguments, 11.5 KB: 4.7 us a launch with 48 as with 160)
-constexpr int kChainMax = 192;          // largest m whose products run as one chain in one workgroup's LDS
+// Largest m whose products run as one chain in one workgroup: 128, or 192 where at least 96 matrices are larger than 128.  One chain of
+// a group of three takes 81 us at m = 192 however few they are (27 us at 128), the launches tile by tile 7 us each for a dozen
+// matrices and 25 us each for the 205 of the default model.
+constexpr int kChainMax = 192, kChainFew = 128, kChainMany = 96;
+constexpr double kLift[3] = {1.0, 12.0, 150.0};     // fp32 results, 16-bit results, Muon
 constexpr float kGrowth = 1024.f;       // largest singular value that a polynomial may make of one in [0, 1]
 
 struct StepExp { int x, s, q, w, p; };  // scale exponents of X (a group's first step), S, Q, W, P
@@ -47,7 +52,7 @@ struct OrthJob {                        // device copy of one matrix's job
   double* part;
   int n_part, rows, cols, m, mp, mk;    // mp: m padded as rows, mk: m padded as the K axis
   int rp, cp, rk, ck;                   // rows / cols padded the same two ways
-  int wide, aligned;
+  int wide, aligned, chained;
   float scale, in_scale;
   StepExp e[kMaxSteps];
 };
@@ -127,6 +132,7 @@ __global__ __launch_bounds__(256) void orth_setup_k(SetupArgs a) {
     o->rows = j.rows; o->cols = j.cols; o->m = j.rows < j.cols ? j.rows : j.cols;
     o->mp = l.mp; o->mk = l.mk; o->rp = l.rp; o->cp = l.cp; o->rk = l.rk; o->ck = l.ck;
     o->wide = j.rows <= j.cols;
+    o->chained = j.chain >= 0;
     if (j.chain >= 0) a.chain[j.chain] = id;
     const uint64_t bits = (uint64_t)j.src | (uint64_t)j.buf | (uint64_t)j.dst | ((uint64_t)j.cols * (uint64_t)a.elem);
     o->aligned = (bits & (uint64_t)(4 * a.elem - 1)) == 0;        // four elements at a time: every row starts on that boundary
@@ -475,7 +481,7 @@ __global__ __launch_bounds__(256, NBUF * R > 4 ? 1 : 2) void orth_gemm_k(GemmArg
   } else if constexpr (KIND == K_NEXT) {
     A = j.w; ea = e.w; B = j.q[a.i & 1]; eb = e.q; eo = j.e[a.step + 1].s; out = j.s;
   } else {
-    const unsigned char* P = a.i == 0 && j.m > kChainMax ? j.q[0] : j.p[j.m > kChainMax ? a.i & 1 : 0];
+    const unsigned char* P = a.i == 0 && !j.chained ? j.q[0] : j.p[j.chained ? 0 : a.i & 1];
     const unsigned char* X = j.wide ? j.t[a.parity] : j.n[a.parity];
     A = j.wide ? P : X; B = j.wide ? X : P;
     arp = j.rp; brp = j.cp;
@@ -951,7 +957,7 @@ struct OrthPlan {
   int n_chain[kChainMax / 32 + 1];        // chained matrices by mk / 32
   int64_t part_b;
   int k_gram, k_m, k_fin;        // mean number of K slots of a tile's product: X X^T, m x m products, P X
-  int tile_sym, tile_fin, pad;
+  int tile_sym, tile_fin, pad, chain_max;
   Groups g;
 };
 
@@ -987,14 +993,16 @@ int make_plan(const mpose_orth_job* jobs, int n_jobs, const mpose_orth_options* 
     if (!(bx <= kGrowth)) return MPOSE_EINVAL;
   }
   p = OrthPlan{};
-  p.g = make_groups(o->steps, o->a, muon ? 150.0 : 12.0);
+  p.g = make_groups(o->steps, o->a, kLift[muon ? 2 : o->dtype == 0 ? 0 : 1]);
   // Tile sizes: 128 reads half as many operand bytes per product but wants enough tiles to fill the chip, and matrices that it does not pad by
   // more than an eighth.  4096 x 4096: symmetric products 252 us with 64, 196 with 128, P X 472 and 365; 1024 x 1024 (36 tiles): 13 and 28 us.
   int64_t area[2][2] = {}, count[2][2] = {};        // [64, 128][symmetric, P X]
+  int n_between = 0;
   for (int i = 0; i < n_jobs; ++i) {
     const int rows = jobs[i].rows, cols = jobs[i].cols;
     if (rows < 1 || cols < 1 || rows > (1 << 21) || cols > (1 << 21) || (int64_t)rows * cols > (1 << 28)) return MPOSE_EINVAL;
     const int64_t m = rows < cols ? rows : cols;
+    if (m > kChainFew && m <= kChainMax) ++n_between;
     for (int t = 0; t < 2; ++t) {
       const int64_t T = 64 << t, tm = (m + T - 1) / T, tf = ((rows + T - 1) / T) * ((cols + T - 1) / T);
       count[t][0] += tm * (tm + 1) / 2; count[t][1] += tf;
@@ -1003,6 +1011,7 @@ int make_plan(const mpose_orth_job* jobs, int n_jobs, const mpose_orth_options* 
   }
   p.tile_sym = count[1][0] >= 384 && area[1][0] * 8 <= area[0][0] * 9 ? 128 : 64;
   p.tile_fin = count[1][1] >= 192 && area[1][1] * 8 <= area[0][1] * 9 ? 128 : 64;
+  p.chain_max = n_between >= kChainMany ? kChainMax : kChainFew;
   p.pad = p.tile_sym > p.tile_fin ? p.tile_sym : p.tile_fin;
   int64_t body = 0, s_gram = 0, s_m = 0, s_fin = 0;
   for (int i = 0; i < n_jobs; ++i) {
@@ -1015,7 +1024,7 @@ int make_plan(const mpose_orth_job* jobs, int n_jobs, const mpose_orth_options* 
     const int64_t tm = (m + p.tile_sym - 1) / p.tile_sym, ns = tm * (tm + 1) / 2;
     const int64_t nf = (int64_t)((rows + p.tile_fin - 1) / p.tile_fin) * ((cols + p.tile_fin - 1) / p.tile_fin);
     p.n_sym += ns;
-    if (m <= kChainMax) p.n_chain[l.mk / 32] += 1;
+    if (m <= p.chain_max) p.n_chain[l.mk / 32] += 1;
     else { p.n_big += ns; s_m += ns * (l.mk / 32); }
     p.n_fin += nf;
     s_gram += ns * ((rows < cols ? l.ck : l.rk) / 32);
@@ -1093,7 +1102,7 @@ int run(const mpose_orth_job* jobs, int n_jobs, const mpose_orth_options* o, boo
     split += ((j.rows + 63) / 64) * ((j.cols + 63) / 64);
     const int m = j.rows < j.cols ? j.rows : j.cols, tm = (m + p.tile_sym - 1) / p.tile_sym;
     sym += tm * (tm + 1) / 2;
-    if (m <= kChainMax) j.chain = chain[l.mk / 32]++;
+    if (m <= p.chain_max) j.chain = chain[l.mk / 32]++;
     else big += tm * (tm + 1) / 2;
     fin += ((j.rows + p.tile_fin - 1) / p.tile_fin) * ((j.cols + p.tile_fin - 1) / p.tile_fin);
     if (sa.n == kSetupJobs || i == n_jobs - 1) {

@@ -352,3 +352,21 @@ def test_large_matrices(shape):
     assert float((got.double() - want).norm() / want.norm()) <= TOL_FLAT
     bf = orthogonalize(g.bfloat16())
     assert float((bf.double() - want).norm() / want.norm()) <= 2.0 ** -7       # (the input's own rounding, 2^-9 of each element, lifted where s is small)
+
+
+def test_many_matrices_between_128_and_192():
+    """A set of at least 96 of them runs each one's products as a chain in one workgroup; fewer run tile by tile: both near the formula."""
+    from margipose_amd.train_helpers import orthogonalize
+    gen = torch.Generator().manual_seed(17)
+    sizes = [129, 160, 161, 191, 192, 150]
+    mats = [torch.randn(sizes[i % 6], 200 + i % 37, generator=gen).cuda() for i in range(100)] + [torch.randn(250, sizes[i], generator=gen).cuda() for i in range(6)]
+    for abc, steps in ((ABC, 5), ((1.5, -0.5, 0.0), 9)):
+        many, few = orthogonalize(mats, steps=steps, coefficients=abc), orthogonalize(mats[:12], steps=steps, coefficients=abc)
+        for i in list(range(12)) + [57, 99, 100, 105]:
+            want = _exact(mats[i], steps, abc)
+            assert _rel(many[i], want) <= TOL_ANY, i
+            if i < 12:
+                assert _rel(few[i], want) <= TOL_ANY, i
+    half = orthogonalize([m.bfloat16() for m in mats])
+    for i in (0, 1, 2, 3, 4, 5, 103):
+        assert _rel(half[i], _exact(mats[i].bfloat16())) <= TOL_ANY + 2.0 ** -8
