@@ -288,6 +288,8 @@ def _pointers(tensors):
 
 
 def _orth_options(steps, coefficients, eps, dtype, nesterov=False):
+    if not isinstance(steps, int) or not 1 <= steps <= 24:
+        raise _lib.MposeError('Newton-Schulz: refused: 1..24 steps, got %r' % (steps,))
     try:
         a, b, c = (float(v) for v in coefficients)
     except (TypeError, ValueError):
