@@ -9,8 +9,8 @@
 // In a group the rounding of S is lifted by a^2 a step where s is small, so a group is as long as a^2 to the power (length - 1) stays below
 // a limit (kLift): 1 for mpose_orthogonalize's fp32 results (X on every step for the customary a = 3.4445), 12 for 16-bit results (groups of
 // 2, 2, 1: their rounding hides the difference), 150 for mpose_muon_step (3, 2), whose result is a small part of a weight.  Relative error
-// against float64, fp32 result: 17 x 128 1.2e-6, 2.0e-6 and 2.4e-6; 128 x 1152 1.1e-6, 1.4e-6 and 3.4e-6 (X on every step in plain fp32:
-// 1.1e-6, 1.4e-6); one group of five 1e-4.  Visits of the long axis: 5, 3, 2.
+// against float64 (plain fp32 products: 1.1e-6 at 17 x 128, 1.4e-6 at 128 x 1152): X on every step 0.9e-6 and 1.0e-6; 3, 2: 1.4e-6 and
+// 3.4e-6; 2, 2, 1 on twelve 17 x 128: up to 2.2e-6.  One group of five, in a model of the arithmetic: 1e-4.  Visits of the long axis: 5, 3, 2.
 //
 // Arithmetic: like the convolutions (three fp16 products of two-way split operands, x * 2^k = h + l: 22 bits), but the scale
 // exponents come from a bound, not from a measurement: |x_ij| <= |X|_2, and a scalar recursion bounds |X|_2, |S|_2, |Q|_2 from the
@@ -35,8 +35,8 @@ constexpr int kMaxSteps = 24;
 constexpr int kChunk = 4096;            // elements per workgroup of the momentum / norm pass
 constexpr int kSetupJobs = 160;         // jobs per set-up launch (they travel as kernel arguments, 11.5 KB: 4.7 us a launch with 48 as with 160)
 // Largest m whose products run as one chain in one workgroup: 128, or 192 where at least 96 matrices are larger than 128.  One chain of
-// a group of three takes 81 us at m = 192 however few they are (27 us at 128), the launches tile by tile 7 us each for a dozen
-// matrices and 25 us each for the 205 of the default model.
+// a group of three takes 81 us at m = 192 however few they are, the nine launches tile by tile 7 us each for a dozen matrices and 25 us
+// each for the 205 of the default model.
 constexpr int kChainMax = 192, kChainFew = 128, kChainMany = 96;
 constexpr double kLift[3] = {1.0, 12.0, 150.0};     // fp32 results, 16-bit results, Muon
 constexpr float kGrowth = 1024.f;       // largest singular value that a polynomial may make of one in [0, 1]
@@ -963,7 +963,7 @@ struct OrthPlan {
 
 // How a launch of n tiles with k slots each fills the chip.  A CU holds two 128-tiles or three 64-tiles at a time; the tiles left after
 // the full rounds are split along K over the idle places when that saves more than the join costs: over 32 slots of 0.3 us (a lone
-// 64-tile) to 0.7 us, against 7 to 10 us.  1024 x 4096, X X^T (136 tiles, 128 slots): 44 us whole, 31 split in five and joined; at 32
+// 64-tile) to 0.7 us, against 7 to 10 us.  1024 x 4096, X X^T (136 tiles, 128 slots): 44 us whole, 29 split in five and joined; at 32
 // slots 13 whole, 17 split.
 struct Fill { int n_main, split; };
 Fill fill_for(int64_t n, int k, int tile) {
@@ -995,7 +995,7 @@ int make_plan(const mpose_orth_job* jobs, int n_jobs, const mpose_orth_options* 
   p = OrthPlan{};
   p.g = make_groups(o->steps, o->a, kLift[muon ? 2 : o->dtype == 0 ? 0 : 1]);
   // Tile sizes: 128 reads half as many operand bytes per product but wants enough tiles to fill the chip, and matrices that it does not pad by
-  // more than an eighth.  4096 x 4096: symmetric products 252 us with 64, 196 with 128, P X 472 and 365; 1024 x 1024 (36 tiles): 13 and 28 us.
+  // more than an eighth.  4096 x 4096: symmetric products 252 us with 64, 196 with 128, P X 472 and 365; 1024 x 1024 (136 and 36 tiles): 13 and 31 us.
   int64_t area[2][2] = {}, count[2][2] = {};        // [64, 128][symmetric, P X]
   int n_between = 0;
   for (int i = 0; i < n_jobs; ++i) {
